@@ -72,8 +72,9 @@ def activations(rows, cols, gen):
 
 
 def codes_of(x, axis):
-    """The codes, and their scales: x / scale in 64 bits, as a quotient next to a half step may be rounded past it in 32."""
-    scale = (x.abs().amax(axis, keepdim=True) / 127).clamp(min=TINY)
+    """The codes, and their scales: both quotients in 64 bits (the scale then rounded), as one next to a half step may be
+    rounded past it in 32."""
+    scale = (x.abs().amax(axis, keepdim=True).double() / 127).float().clamp(min=TINY)
     return torch.round(x.double() / scale).clamp(-127, 127).float(), scale
 
 
