@@ -251,6 +251,67 @@ int pf_gemm_bias_gelu_noalloc(int device, pf_dtype dtype, const pf_tile *tile, i
                               float scale_b, void *stream, unsigned *status_out, char *err,
                               size_t err_len);
 
+/* ---- 8-bit operators ---------------------------------------------------------------------- */
+/* The fused product served from 8-bit integers, and trained through with activations kept in 8 bits.  No
+ * counterpart in the reference.  Codes are int8 with one fp32 scale for each token (row) or channel (column).
+ *
+ * Conventions of this section
+ *   - No pf_ctx: each call names its device and stream (NULL = the CUDA default stream; a stream of another
+ *     device is refused with PF_EINVAL).  Operands and workspaces are the caller's, nothing is allocated and no
+ *     call waits for the GPU, so calls may be captured into a graph (make the first call of each kind on a
+ *     device before that) and made from several threads.  Calls that overlap on the GPU need workspaces of
+ *     their own, and so do two captured graphs that may.
+ *   - Matrices are row-major; ld* are row strides in elements, at least the row's length.
+ *   - rows, M = 0 (no tokens) is a call that writes nothing, or the zero sums that are over tokens.
+ *   - `err` (may be NULL) receives a message of at most `err_len` bytes on failure.
+ *   - Kernel-side waits are bounded by 4 s; one that ran out sets a bit that pf_ops8_status reads. */
+
+/* Codes and scales of X (PF_F32 or PF_BF16), rows x cols:
+ *     scale = max(max |x| / 127, 2^-126),  code = rint(x / scale), the real quotient rounded once
+ * over each row (axis 1: a scale for each token, scale [rows]) or column (axis 0: for each channel, scale [cols]).
+ * Where a row (column) holds an infinity or NaN its scale is NaN and its codes 0. */
+int pf_quantize_s8(int device, pf_dtype src, int rows, int cols, const void *X, long long ldx, int axis,
+                   signed char *codes, long long ld_codes, float *scale, void *stream, char *err, size_t err_len);
+
+/* X = code * scale in fp32, rounded once to dst (PF_F32 or PF_BF16). */
+int pf_dequantize_s8(int device, int rows, int cols, const signed char *codes, long long ld_codes, const float *scale,
+                     int axis, pf_dtype dst, void *X, long long ldx, void *stream, char *err, size_t err_len);
+
+/* C[r,c] = f( scale_a[r] * scale_b[c] * sum_k A[r,k] * B[k,c] + bias[c] ), A [M x K] and B [K x N] int8 codes, the
+ * sum exact in 32-bit integers (hence K <= 131071), the rest in fp32, rounded once to `out` (PF_BF16 or PF_F32).
+ * bias may be NULL (none); f is gelu_tanh where `gelu` is nonzero, the identity otherwise. */
+int pf_gemm_s8(int device, int M, int N, int K, const signed char *A, long long lda, const signed char *B,
+               long long ldb, const float *scale_a, const float *scale_b, const float *bias, int gelu, pf_dtype out,
+               void *C, long long ldc, void *stream, char *err, size_t err_len);
+
+/* The forward pass of the bf16 fused product for training: z = A B + bias, C = gelu_tanh(z) in bf16, and in 8 bits
+ * what the backward pass needs instead of A and z:
+ *   a_codes [M x K], a_scale [M]   pf_quantize_s8 of A, a scale for each token (both NULL: not kept)
+ *   grad_codes [M x N]             d = gelu_tanh'(z) as rint(200 d) + 26 (0 .. 252; 255 for NaN): an absolute
+ *                                  error of at most 0.0025, exact where d is 0 or 1
+ * All matrices contiguous and 16-byte aligned, rows multiples of 16 bytes (N and K multiples of 8: PF_ESHAPE). */
+int pf_gemm_bias_gelu_checkpoint(int device, int M, int N, int K, const void *A, const void *B, const float *bias,
+                                 void *C, signed char *a_codes, float *a_scale, unsigned char *grad_codes, void *stream,
+                                 char *err, size_t err_len);
+
+/* Its backward pass from dC [M x N] (bf16), B and the checkpoint:  dz = dC d,  dbias = sum over tokens of dz (fp32),
+ * dA = dz B^T,  dB = A~^T dz with A~ = a_codes a_scale (bf16, fp32 sums).  Besides the results only dz
+ * is rounded to bf16, once; dbias sums the unrounded dz.  Any of dA, dB, dbias may be NULL (not wanted).  The same inputs
+ * give the same bits.  `workspace`: pf_gemm_bias_gelu_backward_workspace(M, N, K) bytes, 256-byte aligned. */
+int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, const void *B,
+                               const signed char *a_codes, const float *a_scale, const unsigned char *grad_codes,
+                               void *dA, void *dB, float *dbias, void *workspace, size_t workspace_bytes, void *stream,
+                               char *err, size_t err_len);
+size_t pf_gemm_bias_gelu_backward_workspace(int M, int N, int K);
+
+/* The derivatives that `count` grad_codes stand for, (code - 26) / 200, in dst (PF_F32 or PF_BF16). */
+int pf_dequantize_gelu_grad(int device, long long count, const unsigned char *codes, pf_dtype dst, void *X,
+                            void *stream, char *err, size_t err_len);
+
+/* Synchronise the device, read and clear the bits of bounded waits that ran out in this section's kernels (0 =
+ * clean; bits as pf_device_status).  Bits of calls on every stream of the device gather in one word. */
+int pf_ops8_status(int device, unsigned *err_word, char *err, size_t err_len);
+
 /* ---- utilities ---------------------------------------------------------------------------- */
 
 /* Bytes of one element of A/B and of C for a dtype (0 for an unknown dtype). */

@@ -7,6 +7,9 @@ attributes.  There is no CPU fallback: without the library or an sm_100 GPU ever
 
     import torch, ptxforge_b200 as pf
     C = pf.gemm_bias_gelu(A, B, bias, dtype="bf16")          # A, B, bias CUDA tensors
+
+The 8-bit operators (ops8.py): the same product served from int8 codes (quantize_s8, gemm_s8), and trained through
+with its activations kept in 8 bits (gemm_bias_gelu_checkpoint, gemm_bias_gelu_backward).
 """
 from __future__ import annotations
 
@@ -31,7 +34,10 @@ SYMBOLS = ("pf_open", "pf_close", "pf_prepare", "pf_bind", "pf_launch", "pf_time
            "pf_device_status", "pf_set_wait_timeout", "pf_last_error", "pf_run_host", "pf_shard_rows",
            "pf_elem_bytes", "pf_out_bytes", "pf_version", "pf_selftest_wait_timeout", "pf_upload", "pf_download",
            "pf_gemm_bias_gelu_noalloc", "pf_prepare_image", "pf_time_cublas",
-           "pf_set_stream_k", "pf_run_host_rows", "pf_set_host_chunks")
+           "pf_set_stream_k", "pf_run_host_rows", "pf_set_host_chunks",
+           "pf_quantize_s8", "pf_dequantize_s8", "pf_gemm_s8", "pf_gemm_bias_gelu_checkpoint",
+           "pf_gemm_bias_gelu_backward", "pf_gemm_bias_gelu_backward_workspace", "pf_dequantize_gelu_grad",
+           "pf_ops8_status")
 
 
 class Tile(ctypes.Structure):
@@ -169,10 +175,22 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.pf_out_bytes.restype = ctypes.c_size_t
         lib.pf_version.restype = ctypes.c_char_p
         lib.pf_selftest_wait_timeout.argtypes = [vp, ctypes.c_ulonglong, ctypes.POINTER(ctypes.c_uint)]
+        f32p, ll, sz, text = vp, ctypes.c_longlong, ctypes.c_size_t, ctypes.c_char_p
+        lib.pf_quantize_s8.argtypes = [i, i, i, i, vp, ll, i, vp, ll, f32p, vp, text, sz]
+        lib.pf_dequantize_s8.argtypes = [i, i, i, vp, ll, f32p, i, i, vp, ll, vp, text, sz]
+        lib.pf_gemm_s8.argtypes = [i, i, i, i, vp, ll, vp, ll, f32p, f32p, f32p, i, i, vp, ll, vp, text, sz]
+        lib.pf_gemm_bias_gelu_checkpoint.argtypes = [i, i, i, i, vp, vp, f32p, vp, vp, f32p, vp, vp, text, sz]
+        lib.pf_gemm_bias_gelu_backward.argtypes = [i, i, i, i, vp, vp, vp, f32p, vp, vp, vp, f32p, vp, sz, vp, text, sz]
+        lib.pf_gemm_bias_gelu_backward_workspace.argtypes = [i, i, i]
+        lib.pf_gemm_bias_gelu_backward_workspace.restype = sz
+        lib.pf_dequantize_gelu_grad.argtypes = [i, ll, vp, i, vp, vp, text, sz]
+        lib.pf_ops8_status.argtypes = [i, ctypes.POINTER(ctypes.c_uint), text, sz]
         for name in ("pf_open", "pf_close", "pf_prepare", "pf_bind", "pf_launch", "pf_time", "pf_attrs",
                      "pf_device_status", "pf_set_wait_timeout", "pf_run_host", "pf_run_host_rows", "pf_shard_rows",
                      "pf_selftest_wait_timeout", "pf_upload", "pf_download", "pf_gemm_bias_gelu_noalloc",
-                     "pf_prepare_image", "pf_time_cublas", "pf_set_stream_k", "pf_set_host_chunks"):
+                     "pf_prepare_image", "pf_time_cublas", "pf_set_stream_k", "pf_set_host_chunks",
+                     "pf_quantize_s8", "pf_dequantize_s8", "pf_gemm_s8", "pf_gemm_bias_gelu_checkpoint",
+                     "pf_gemm_bias_gelu_backward", "pf_dequantize_gelu_grad", "pf_ops8_status"):
             getattr(lib, name).restype = ctypes.c_int
         if path is None:
             _lib = lib
@@ -428,3 +446,7 @@ def gemm_bias_gelu(A, B, bias, C=None, *, dtype: str | None = None, tile=None, s
         stream = torch.cuda.current_stream(A.device)
     ctx.launch(stream)
     return C
+
+
+from .ops8 import (Checkpoint, dequantize_gelu_grad, dequantize_s8, gemm_bias_gelu_backward,  # noqa: E402,F401
+                   gemm_bias_gelu_checkpoint, gemm_s8, ops8_status, quantize_s8)

@@ -9,9 +9,11 @@ reports PF_ENODEV) where no GPU driver is installed.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -31,13 +33,24 @@ def nvcc_path() -> str:
     return found
 
 
-def _sources() -> list[str]:
-    out = []
-    for d in (CSRC, INCLUDE):
-        for name in sorted(os.listdir(d)):
-            if name.endswith((".cu", ".cuh", ".h", ".hpp")):
-                out.append(os.path.join(d, name))
-    return out
+# Translation units of the library, compiled side by side: the fused product's kernels and ABI, and the 8-bit operators'.
+UNITS = ("pf_b200.cu", "ops8.cu")
+OBJ_DIR = os.path.join(ROOT, "build")
+
+
+def _includes(path: str, seen: set | None = None) -> set:
+    """`path` and every header of this repository that it includes."""
+    seen = set() if seen is None else seen
+    if path in seen:
+        return seen
+    seen.add(path)
+    with open(path) as f:
+        names = re.findall(r'^\s*#include\s+"([^"]+)"', f.read(), re.M)
+    for n in names:
+        for d in (CSRC, INCLUDE):
+            if os.path.exists(os.path.join(d, n)):
+                _includes(os.path.join(d, n), seen)
+    return seen
 
 
 def _stale(target: str, deps: list[str]) -> bool:
@@ -47,20 +60,40 @@ def _stale(target: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile libpf_b200.so if any source is newer than it; return its path."""
-    if not force and not _stale(LIB, _sources() + [os.path.abspath(__file__)]):
-        return LIB
-    cmd = [
-        nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
-        "-Xcompiler", "-fPIC,-Wall", "-shared", "-cudart", "static",
-        "-I", INCLUDE, "-I", CSRC, "-Xptxas", "-v",
-        os.path.join(CSRC, "pf_b200.cu"), "-o", LIB + ".tmp",
-    ]
+def _run(cmd: list[str]) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     log = r.stdout + r.stderr
     if r.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + log[-6000:])
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n" + log[-6000:])
+    return log
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile libpf_b200.so if any source is newer than it; return its path."""
+    me = os.path.abspath(__file__)
+    units = {u: os.path.join(CSRC, u) for u in UNITS}
+    deps = {u: sorted(_includes(src)) + [me] for u, src in units.items()}
+    if not force and not _stale(LIB, [d for ds in deps.values() for d in ds]):
+        return LIB
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    objs = {u: os.path.join(OBJ_DIR, u[:-3] + ".o") for u in UNITS}
+
+    def compile_unit(u):
+        log_path = objs[u] + ".ptxas.txt"
+        if not force and os.path.exists(log_path) and not _stale(objs[u], deps[u]):
+            with open(log_path) as f:
+                return f.read()
+        log = _run([nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
+                    "-Xcompiler", "-fPIC,-Wall", "-cudart", "static", "-I", INCLUDE, "-I", CSRC, "-Xptxas", "-v",
+                    "-c", units[u], "-o", objs[u] + ".tmp"])
+        with open(log_path, "w") as f:
+            f.write(log)
+        os.replace(objs[u] + ".tmp", objs[u])
+        return log
+
+    with ThreadPoolExecutor(len(UNITS)) as pool:
+        log = "".join(pool.map(compile_unit, UNITS))
+    _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-cudart", "static", *objs.values(), "-o", LIB + ".tmp"])
     os.replace(LIB + ".tmp", LIB)
     with open(os.path.join(HERE, "libpf_b200.ptxas.txt"), "w") as f:
         f.write(log)

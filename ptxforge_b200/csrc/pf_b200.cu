@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "pf_b200.h"
+#include "host_util.cuh"
 #include "gemm_simt.cuh"
 #include "gemm_simt_tma.cuh"
 #include "gemm_tc.cuh"
@@ -34,12 +35,12 @@
 
 namespace {
 
+using pf::aligned16;
+using pf::DeviceGuard;
+using pf::encode_2d_msg;
+using pf::launch_pdl;
 using pf::TcConfig;
 using pf::TcParams;
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 enum class Path { kNone, kSimt, kTensor, kImage };
 
@@ -83,18 +84,6 @@ struct Variant {
                           int, int, unsigned *, unsigned long long) = nullptr;
 };
 
-// Programmatic dependent launch for the tensor-core kernels: each launch may be scheduled while the previous
-// kernel in the stream finishes; the kernel sets up its barriers and TMEM, then waits (griddepcontrol.wait)
-// for that kernel's completion before any global memory access, so the result is the same as a plain launch.
-// PF_PDL=0 in the environment turns it off (plain launches).
-bool pdl_enabled() {
-  static const bool on = [] {
-    const char *e = std::getenv("PF_PDL");
-    return !(e && e[0] == '0');
-  }();
-  return on;
-}
-
 // Tail split of the 256 x 512 pair kernel (TcParams::tail_split): k steps at the end of each pair's last tile
 // whose second-half MMAs run after the first half's, so that the first half's epilogue overlaps them.
 // PF_TAIL_SPLIT=<steps> in the environment overrides the default (0 turns it off).
@@ -119,24 +108,6 @@ int promote_kb_default() {
     return e ? std::max(0, std::atoi(e)) : 4;
   }();
   return kb;
-}
-
-template <class... Params, class... Args>
-void launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args &&...args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  cfg.numAttrs = 0;
-  if (pdl_enabled()) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-  }
-  cfg.attrs = attr;
-  cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);  // errors surface through cudaGetLastError
 }
 
 template <int DT, int BN, int ST, int KA>
@@ -441,22 +412,6 @@ const char *cu_err(CUresult r) {
   return s ? s : "unknown CUDA driver error";
 }
 
-// The driver's cuTensorMapEncodeTiled.  A function-local static is initialised exactly once, and threads
-// whose first calls race all wait for that one initialisation (C++11 guarantees it), so none can see a
-// half-initialised value.
-EncodeTiledFn get_encode_fn() {
-  static const EncodeTiledFn fn = [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      return reinterpret_cast<EncodeTiledFn>(p);
-    return static_cast<EncodeTiledFn>(nullptr);
-  }();
-  return fn;
-}
-
 }  // namespace
 
 struct pf_ctx {
@@ -529,43 +484,6 @@ int set_err(pf_ctx *c, int code, const char *fmt, ...) {
     if (_e != cudaSuccess) return set_err(ctx, PF_ECUDA, "%s -> %s", #call, cudaGetErrorString(_e));    \
   } while (0)
 
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    cudaGetDevice(&prev);
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    cudaGetDevice(&cur);
-    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-  }
-};
-
-// A 2-D tiled TMA map; on failure a message goes to msg[0..len) (no heap: the no-allocation entry point
-// uses it too).
-int encode_2d_msg(char *msg, size_t len, CUtensorMap *map, CUtensorMapDataType dt, const void *base, uint64_t inner,
-                  uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz) {
-  EncodeTiledFn enc = get_encode_fn();
-  if (!enc) {
-    if (msg && len) snprintf(msg, len, "cuTensorMapEncodeTiled unavailable from the CUDA driver");
-    return PF_ECUDA;
-  }
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, dt, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    if (msg && len)
-      snprintf(msg, len, "cuTensorMapEncodeTiled failed (%d) for a %llux%llu tensor, box %ux%u", (int)r,
-               (unsigned long long)outer, (unsigned long long)inner, box_outer, box_inner);
-    return PF_ECUDA;
-  }
-  return PF_OK;
-}
-
 int encode_2d(pf_ctx *c, CUtensorMap *map, CUtensorMapDataType dt, const void *base, uint64_t inner, uint64_t outer,
               uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz) {
   char msg[200];
@@ -615,8 +533,6 @@ int encode_maps(pf_ctx *c) {
   if ((rc = encode_c_map(c, &c->tmC, c->C, c->M))) return rc;
   return encode_c_tail_map(c, &c->tmCt, c->tmC, c->C, c->M);
 }
-
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // The 3xTF32 kernel's running-sum workspace for `workers` pairs, and the promotion parameters of a launch.
 int set_promotion(pf_ctx *c, int workers, TcParams &p) {
