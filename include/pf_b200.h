@@ -279,10 +279,15 @@ int pf_dequantize_s8(int device, int rows, int cols, const signed char *codes, l
 
 /* C[r,c] = f( scale_a[r] * scale_b[c] * sum_k A[r,k] * B[k,c] + bias[c] ), A [M x K] and B [K x N] int8 codes, the
  * sum exact in 32-bit integers (hence K <= 131071), the rest in fp32, rounded once to `out` (PF_BF16 or PF_F32).
- * bias may be NULL (none); f is gelu_tanh where `gelu` is nonzero, the identity otherwise. */
+ * bias may be NULL (none); f is gelu_tanh where `gelu` is nonzero, the identity otherwise.
+ * Rows of A or B that do not start on 16-byte boundaries (the matrix, or its row stride) are copied to `workspace`
+ * first: pf_gemm_s8_workspace(...) bytes, 256-byte aligned; 0 bytes (NULL) where both fit as they are. */
 int pf_gemm_s8(int device, int M, int N, int K, const signed char *A, long long lda, const signed char *B,
                long long ldb, const float *scale_a, const float *scale_b, const float *bias, int gelu, pf_dtype out,
-               void *C, long long ldc, void *stream, char *err, size_t err_len);
+               void *C, long long ldc, void *workspace, size_t workspace_bytes, void *stream, char *err,
+               size_t err_len);
+size_t pf_gemm_s8_workspace(int M, int N, int K, const signed char *A, long long lda, const signed char *B,
+                            long long ldb);
 
 /* The forward pass of the bf16 fused product for training: z = A B + bias, C = gelu_tanh(z) in bf16, and in 8 bits
  * what the backward pass needs instead of A and z:

@@ -35,8 +35,8 @@ SYMBOLS = ("pf_open", "pf_close", "pf_prepare", "pf_bind", "pf_launch", "pf_time
            "pf_elem_bytes", "pf_out_bytes", "pf_version", "pf_selftest_wait_timeout", "pf_upload", "pf_download",
            "pf_gemm_bias_gelu_noalloc", "pf_prepare_image", "pf_time_cublas",
            "pf_set_stream_k", "pf_run_host_rows", "pf_set_host_chunks",
-           "pf_quantize_s8", "pf_dequantize_s8", "pf_gemm_s8", "pf_gemm_bias_gelu_checkpoint",
-           "pf_gemm_bias_gelu_backward", "pf_gemm_bias_gelu_backward_workspace", "pf_dequantize_gelu_grad",
+           "pf_quantize_s8", "pf_dequantize_s8", "pf_gemm_s8", "pf_gemm_s8_workspace",
+           "pf_gemm_bias_gelu_checkpoint", "pf_gemm_bias_gelu_backward", "pf_gemm_bias_gelu_backward_workspace", "pf_dequantize_gelu_grad",
            "pf_ops8_status")
 
 
@@ -178,7 +178,9 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         f32p, ll, sz, text = vp, ctypes.c_longlong, ctypes.c_size_t, ctypes.c_char_p
         lib.pf_quantize_s8.argtypes = [i, i, i, i, vp, ll, i, vp, ll, f32p, vp, text, sz]
         lib.pf_dequantize_s8.argtypes = [i, i, i, vp, ll, f32p, i, i, vp, ll, vp, text, sz]
-        lib.pf_gemm_s8.argtypes = [i, i, i, i, vp, ll, vp, ll, f32p, f32p, f32p, i, i, vp, ll, vp, text, sz]
+        lib.pf_gemm_s8.argtypes = [i, i, i, i, vp, ll, vp, ll, f32p, f32p, f32p, i, i, vp, ll, vp, sz, vp, text, sz]
+        lib.pf_gemm_s8_workspace.argtypes = [i, i, i, vp, ll, vp, ll]
+        lib.pf_gemm_s8_workspace.restype = sz
         lib.pf_gemm_bias_gelu_checkpoint.argtypes = [i, i, i, i, vp, vp, f32p, vp, vp, f32p, vp, vp, text, sz]
         lib.pf_gemm_bias_gelu_backward.argtypes = [i, i, i, i, vp, vp, vp, f32p, vp, vp, vp, f32p, vp, sz, vp, text, sz]
         lib.pf_gemm_bias_gelu_backward_workspace.argtypes = [i, i, i]

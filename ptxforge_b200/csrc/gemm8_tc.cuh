@@ -1,0 +1,558 @@
+// gemm8_tc.cuh -- the products of the 8-bit operators on the 5th-generation tensor cores.
+//
+// Every one of them is  out[t][c] = f( sum_r T(t, r) W(r, c) )  with out row-major: t runs over tokens (for dB: over the
+// input's columns), c over channels.  The tensor cores compute the transpose: UMMA rows are channels, UMMA columns
+// tokens.  Then a TMEM lane is a channel, so
+//   * a warp's store of one token is 32 neighbouring channels: whole sectors from registers, with no staging in shared
+//     memory, no tensor map and no rule on out's alignment or row length;
+//   * what belongs to a channel (its scale, its bias) sits in a register of its lane;
+//   * few tokens make a narrow MMA (N = 16) instead of a mostly empty one, and little shared memory.
+// Operands come by TMA in either order: K-major (the summed index contiguous) or MN-major, as they lie in memory; what a
+// tile reaches past a matrix's edge is filled with zeros.  Element types: bf16 (fp32 sums) or int8 (int32 sums, exact).
+//
+//   gemm8_pair  256 channels x 256 tokens a CTA pair (.cta_group::2), persistent, two accumulators: tile i's epilogue
+//               runs beside tile i+1's MMAs.  For products with enough tiles to fill the GPU.
+//   gemm8_one   128 channels x 16..256 tokens a CTA, the sum split over a cluster of up to 8 CTAs whose accumulators are
+//               added through distributed shared memory, in rank order.  For few tokens, where the bytes of W are
+//               what counts, and for small products.
+#pragma once
+
+#include "gemm_tc.cuh"
+#include "ops8_epilogue.cuh"
+
+namespace pf {
+
+// kElem: bytes of an element.  kWK: W lies as [c][r] (K-major), else as [r][c].  kTK: T lies as [t][r], else as [r][t].
+// kTokens: tokens that this CTA loads.
+template <int kElem, bool kWK, bool kTK, int kTokens, int kAtoms>
+struct Operands {
+  static constexpr int ELEM = kElem;
+  static constexpr int TOKENS = kTokens;
+  static constexpr int CHANNELS = 128;
+  static constexpr int ATOM = 128 / kElem;        // elements of one 128-byte swizzle row
+  static constexpr int BK = kAtoms * ATOM;        // summed index per stage
+  static constexpr int UMMA_K = 32 / kElem;
+  static constexpr int STEPS = BK / UMMA_K;       // MMAs per stage
+  static constexpr int W_BYTES = kAtoms * CHANNELS * 128, T_BYTES = kAtoms * TOKENS * 128;
+  static constexpr int STAGE_BYTES = W_BYTES + T_BYTES;
+  static constexpr bool W_K = kWK, T_K = kTK;
+  // TMA boxes: (inner, outer) elements
+  static constexpr int W_BOX0 = ATOM, W_BOX1 = kWK ? CHANNELS : BK, T_BOX0 = ATOM, T_BOX1 = kTK ? TOKENS : BK;
+  static_assert(kTK || TOKENS % ATOM == 0, "MN-major tokens come in whole 128-byte rows");
+  static_assert(W_BOX1 <= 256 && T_BOX1 <= 256, "TMA box limit");
+
+  template <bool kK, int kRows, class Load>
+  static __device__ __forceinline__ void load(uint8_t *dst, int at, int kb, Load one) {
+    if constexpr (kK) {
+#pragma unroll
+      for (int a = 0; a < kAtoms; ++a) one(dst + a * kRows * 128, kb * BK + a * ATOM, at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRows / ATOM; ++j) one(dst + j * BK * 128, at + j * ATOM, kb * BK);
+    }
+  }
+  template <bool kK, int kRows>
+  static __device__ __forceinline__ uint64_t desc(uint32_t addr, int step) {
+    constexpr int PER_ATOM = ATOM / UMMA_K;
+    if constexpr (kK)
+      return smem_desc(addr + (step / PER_ATOM) * kRows * 128 + (step % PER_ATOM) * 32, 16, 1024, kSwizzle128B);
+    else
+      return smem_desc(addr + step * UMMA_K * 128, BK * 128, 1024, kSwizzle128B);
+  }
+  static constexpr uint32_t idesc(uint32_t M, uint32_t N) {
+    // bf16: formats 1, fp32 sums (bits 4-5: 1); int8: signed formats 1, int32 sums (bits 4-5: 2)
+    const uint32_t d = instr_desc(1u, 1u, kWK ? 0u : 1u, kTK ? 0u : 1u, M, N);
+    return kElem == 2 ? d : (d & ~(3u << 4)) | (2u << 4);
+  }
+};
+
+struct Gemm8Params {
+  int channels, tokens;          // out's columns and rows
+  int c_tiles, t_tiles, k_blocks;
+  int group;                     // gemm8_pair: channel tiles that the raster walks before the next token tile
+  int stages;                    // gemm8_one: pipeline depth, by the shared memory given
+  unsigned *status;
+  unsigned long long timeout_ns;
+};
+
+// ------------------------------------------------------------------------------------------------
+// epilogues: one object a lane, for its channel
+// ------------------------------------------------------------------------------------------------
+template <class Out>
+struct EpilogueS8 {
+  struct Args {
+    const float *sa, *sb, *bias;  // bias may be null
+    Out *out;
+    long long ld;
+    int gelu;
+  };
+  const Args &a;
+  const int c;
+  const bool inside;
+  float sb, bias;
+  __device__ __forceinline__ EpilogueS8(const Args &args, int channel, int channels)
+      : a(args), c(channel), inside(channel < channels) {
+    sb = inside ? __ldg(a.sb + c) : 0.f;
+    bias = inside && a.bias ? __ldg(a.bias + c) : 0.f;
+  }
+  static __device__ __forceinline__ float token(const Args &a, int t) { return __ldg(a.sa + t); }
+  static __device__ __forceinline__ uint32_t add(uint32_t x, uint32_t y) { return x + y; }
+  __device__ __forceinline__ void put(uint32_t sum, int t, float sa) const {
+    float x = fmaf(static_cast<float>(static_cast<int>(sum)), sa * sb, bias);
+    if (a.gelu) x = gelu_of(x);
+    if (inside) a.out[t * a.ld + c] = from_f32<Out>(x);
+  }
+};
+
+struct EpilogueF32Sum {
+  static __device__ __forceinline__ uint32_t add(uint32_t x, uint32_t y) {
+    return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+  }
+};
+
+struct EpilogueCheckpoint : EpilogueF32Sum {
+  struct Args {
+    const float *bias;
+    __nv_bfloat16 *out;
+    uint8_t *codes;
+    long long ld;
+  };
+  const Args &a;
+  const int c;
+  const bool inside;
+  float bias;
+  __device__ __forceinline__ EpilogueCheckpoint(const Args &args, int channel, int channels)
+      : a(args), c(channel), inside(channel < channels) {
+    bias = inside ? __ldg(a.bias + c) : 0.f;
+  }
+  static __device__ __forceinline__ float token(const Args &, int) { return 0.f; }
+  __device__ __forceinline__ void put(uint32_t sum, int t, float) const {
+    const Gelu g = gelu_and_grad(__uint_as_float(sum) + bias);
+    if (inside) {
+      a.out[t * a.ld + c] = __float2bfloat16_rn(g.y);
+      a.codes[t * a.ld + c] = static_cast<uint8_t>(grad_code(g.d));
+    }
+  }
+};
+
+struct EpilogueBf16 : EpilogueF32Sum {
+  struct Args {
+    const float *token_scale;  // null, or a token's row is divided by its m (split_scale)
+    __nv_bfloat16 *out;
+    long long ld;
+  };
+  const Args &a;
+  const int c;
+  const bool inside;
+  __device__ __forceinline__ EpilogueBf16(const Args &args, int channel, int channels)
+      : a(args), c(channel), inside(channel < channels) {}
+  static __device__ __forceinline__ float token(const Args &a, int t) {
+    return a.token_scale ? __fdiv_rn(1.f, split_scale(__ldg(a.token_scale + t)).m) : 1.f;
+  }
+  __device__ __forceinline__ void put(uint32_t sum, int t, float inv_m) const {
+    if (inside) a.out[t * a.ld + c] = __float2bfloat16_rn(__uint_as_float(sum) * inv_m);
+  }
+};
+
+// 32 tokens from t0 on: lane j holds token t0 + j's scalar.
+template <class Epi>
+__device__ __forceinline__ void put32(const Epi &e, const typename Epi::Args &args, const uint32_t (&v)[32], int t0,
+                                      int tokens, int lane) {
+  const float mine = t0 + lane < tokens ? Epi::token(args, t0 + lane) : 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float s = __shfl_sync(0xffffffffu, mine, j);
+    if (t0 + j < tokens) e.put(v[j], t0 + j, s);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// one CTA a tile, the sum split over a cluster
+// ------------------------------------------------------------------------------------------------
+constexpr int kOneThreads = 192;
+constexpr int kOneMaxStages = 16;
+
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <class Op, class Epi>
+__global__ void __launch_bounds__(kOneThreads)
+    gemm8_one(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const Gemm8Params p,
+              const typename Epi::Args args) {
+  constexpr int TOKENS = Op::TOKENS;
+  constexpr int TMEM_COLS = TOKENS < 32 ? 32 : TOKENS;
+  constexpr uint32_t IDESC = Op::idesc(128, TOKENS);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ uint64_t full[kOneMaxStages], empty[kOneMaxStages], done;
+  __shared__ uint32_t tmem_holder;
+  __shared__ int abort_word;
+  volatile int *abort_flag = &abort_word;
+  uint8_t *sW = smem, *sT = smem + p.stages * Op::W_BYTES;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t splits;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+  const uint32_t rank = cluster_ctarank();
+  const int c0 = static_cast<int>(blockIdx.x / splits) * 128, t0 = static_cast<int>(blockIdx.y) * TOKENS;
+  // this CTA's share of the sum
+  const int kb0 = static_cast<int>(static_cast<long long>(p.k_blocks) * rank / splits);
+  const int kb1 = static_cast<int>(static_cast<long long>(p.k_blocks) * (rank + 1) / splits);
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmT);
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_holder, TMEM_COLS);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  auto fail = [&](unsigned bit) {
+    atomicOr(p.status, bit);
+    *abort_flag = 1;
+  };
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, p.timeout_ns, abort_flag)) {
+          fail(kErrProducerWait);
+          ok = false;
+          break;
+        }
+        uint64_t *bar = &full[stage];
+        mbar_arrive_expect_tx(bar, Op::STAGE_BYTES);
+        Op::template load<Op::W_K, 128>(sW + stage * Op::W_BYTES, c0, kb, [&](uint8_t *dst, int x, int y) {
+          tma_load_2d(dst, &tmW, bar, x, y);
+        });
+        Op::template load<Op::T_K, TOKENS>(sT + stage * Op::T_BYTES, t0, kb, [&](uint8_t *dst, int x, int y) {
+          tma_load_2d(dst, &tmT, bar, x, y);
+        });
+        ++issued;
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) {
+        // Loads in flight land before the CTA may exit (bounded).
+        for (int s = 0; s < p.stages && s < issued; ++s) {
+          const uint32_t ph = (s < stage) ? phase : (phase ^ 1u);
+          volatile int no_abort = 0;
+          if (!mbar_wait(&full[s], ph, p.timeout_ns, &no_abort)) atomicOr(p.status, kErrTeardownWait);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, p.timeout_ns, abort_flag)) {
+          fail(kErrMmaWait);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t w = smem_u32(sW + stage * Op::W_BYTES), t = smem_u32(sT + stage * Op::T_BYTES);
+#pragma unroll
+        for (int i = 0; i < Op::STEPS; ++i) {
+          const uint64_t wd = Op::template desc<Op::W_K, 128>(w, i), td = Op::template desc<Op::T_K, TOKENS>(t, i);
+          const uint32_t accumulate = (kb != kb0 || i != 0) ? 1u : 0u;
+          if constexpr (Op::ELEM == 2) tc_mma_f16(tmem, wd, td, IDESC, accumulate);
+          else tc_mma_i8(tmem, wd, td, IDESC, accumulate);
+        }
+        tc_commit(&empty[stage]);
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      tc_commit(&done);  // every MMA complete: the sums are in TMEM, and no stage is read any more
+      volatile int no_abort = 0;
+      if (!mbar_wait(&done, 0, p.timeout_ns, &no_abort)) atomicOr(p.status, kErrTeardownWait);
+    }
+  } else {
+    const int q = warp & 3;
+    const int c_local = q * 32 + lane;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    const Epi epi(args, c0 + c_local, p.channels);
+    const bool waited = mbar_wait(&done, 0, p.timeout_ns, abort_flag);
+    if (!__all_sync(0xffffffffu, waited)) {
+      if (lane == 0) fail(kErrEpilogueWait);
+    } else {
+      tc_fence_after();
+      uint32_t *mine = reinterpret_cast<uint32_t *>(smem) + c_local;  // [token][128 channels], where the stages were
+#pragma unroll 1
+      for (int b = 0; b < (TOKENS + 31) / 32; ++b) {
+        if (t0 + b * 32 >= p.tokens) break;
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(t_row + b * 32, v);
+        tmem_ld_wait();
+        if (splits == 1) {
+          put32(epi, args, v, t0 + b * 32, min(p.tokens, t0 + TOKENS), lane);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (b * 32 + j < TOKENS) mine[(b * 32 + j) * 128] = v[j];
+        }
+      }
+    }
+  }
+  if (splits > 1) {
+    __syncwarp();
+    cluster_sync();  // every CTA's sums are in its shared memory
+    if (warp >= 2) {
+      const int c_local = (warp & 3) * 32 + lane;
+      const Epi epi(args, c0 + c_local, p.channels);
+      const uint32_t base = smem_u32(smem) + c_local * 4;
+      const int n = min(TOKENS, p.tokens - t0);
+      for (int t = static_cast<int>(rank); t < n; t += static_cast<int>(splits)) {
+        uint32_t sum = ld_cluster(mapa_shared(base + t * 512, 0));
+        for (uint32_t s = 1; s < splits; ++s) sum = Epi::add(sum, ld_cluster(mapa_shared(base + t * 512, s)));
+        epi.put(sum, t0 + t, Epi::token(args, t0 + t));
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // nobody leaves while its shared memory may be read
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// CTA pairs
+// ------------------------------------------------------------------------------------------------
+// Consecutive tiles walk down `group` channel tiles, then across the token tiles, so pairs that run at the same time
+// share both operands' panels in L2.
+__device__ __forceinline__ void pair_tile(int i, const Gemm8Params &p, int &ct, int &tt) {
+  const int per_group = p.group * p.t_tiles;
+  const int g = i / per_group, first = g * p.group;
+  const int rows = min(p.c_tiles - first, p.group);
+  const int r = i - g * per_group;
+  ct = first + r % rows;
+  tt = r / rows;
+}
+
+template <class Op, int kStages>
+struct PairConfig {
+  static constexpr int STAGES = kStages;
+  static constexpr int EPI_WARPS = 4;
+  static constexpr int THREADS = 64 + EPI_WARPS * 32;
+  static constexpr int NUM_BARS = 2 * STAGES + 4 + 1;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * Op::STAGE_BYTES + NUM_BARS * 8 + 16;
+  static constexpr uint32_t IDESC = Op::idesc(256, 256);
+  static_assert(Op::TOKENS == 128, "each CTA of a pair supplies 128 tokens");
+  static_assert(SMEM_BYTES <= 232448, "shared memory per block exceeds the sm_100 opt-in limit");
+};
+
+template <class Op, class Epi, int kStages>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStages>::THREADS, 1)
+    gemm8_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const Gemm8Params p,
+               const typename Epi::Args args) {
+  using Cfg = PairConfig<Op, kStages>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *sW = smem, *sT = smem + Cfg::STAGES * Op::W_BYTES;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Cfg::STAGES * Op::STAGE_BYTES);  // leader: both CTAs' bytes landed
+  uint64_t *empty = full + Cfg::STAGES;                                                 // both: the stage was read
+  uint64_t *tfull = empty + Cfg::STAGES;                                                // both: accumulator ready
+  uint64_t *tempty = tfull + 2;                                                         // leader: accumulator drained
+  uint64_t *drain = tempty + 2;                                                         // leader: all MMAs complete
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = p.c_tiles * p.t_tiles;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmT);
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * Cfg::EPI_WARPS);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_holder, 512);
+    tmem_relinquish_pair();
+    tc_fence_before();
+  }
+  cluster_sync();  // both CTAs' barriers exist before anything arrives on them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  auto fail = [&](unsigned bit) {
+    atomicOr(p.status, bit);
+    *abort_flag = 1;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      bool ok = true;
+      for (int i = pair; ok && i < tiles; i += pairs) {
+        int ct, tt;
+        pair_tile(i, p, ct, tt);
+        const int c0 = ct * 256 + static_cast<int>(rank) * 128, t0 = tt * 256 + static_cast<int>(rank) * 128;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, p.timeout_ns, abort_flag)) {
+            fail(kErrProducerWait);
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * Op::STAGE_BYTES);
+          if (issued == 0) grid_dependency_wait();
+          const uint32_t bar = pair_leader_addr(smem_u32(&full[stage]));
+          Op::template load<Op::W_K, 128>(sW + stage * Op::W_BYTES, c0, kb, [&](uint8_t *dst, int x, int y) {
+            tma_load_2d_pair(dst, &tmW, bar, x, y);
+          });
+          Op::template load<Op::T_K, 128>(sT + stage * Op::T_BYTES, t0, kb, [&](uint8_t *dst, int x, int y) {
+            tma_load_2d_pair(dst, &tmT, bar, x, y);
+          });
+          ++issued;
+          if (++stage == Cfg::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok && rank == 0) {
+        // Loads in flight land before the pair may exit (bounded).
+        for (int s = 0; s < Cfg::STAGES && s < issued; ++s) {
+          const uint32_t ph = (s < stage) ? phase : (phase ^ 1u);
+          volatile int no_abort = 0;
+          if (!mbar_wait(&full[s], ph, p.timeout_ns, &no_abort)) atomicOr(p.status, kErrTeardownWait);
+        }
+      }
+    }
+    grid_launch_dependents();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      for (int i = pair; ok && i < tiles; i += pairs) {
+        if (!mbar_wait_cluster(&tempty[acc], acc_phase ^ 1u, p.timeout_ns, abort_flag)) {
+          fail(kErrMmaWait);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(acc * 256);
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(&full[stage], phase, p.timeout_ns, abort_flag)) {
+            fail(kErrMmaWait);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t w = smem_u32(sW + stage * Op::W_BYTES), t = smem_u32(sT + stage * Op::T_BYTES);
+#pragma unroll
+          for (int k = 0; k < Op::STEPS; ++k) {
+            const uint64_t wd = Op::template desc<Op::W_K, 128>(w, k), td = Op::template desc<Op::T_K, 128>(t, k);
+            const uint32_t accumulate = (kb != 0 || k != 0) ? 1u : 0u;
+            if constexpr (Op::ELEM == 2) tc_mma_f16_pair(d, wd, td, Cfg::IDESC, accumulate);
+            else tc_mma_i8_pair(d, wd, td, Cfg::IDESC, accumulate);
+          }
+          tc_commit_pair_mc(&empty[stage], 0x3);
+          if (++stage == Cfg::STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair_mc(&tfull[acc], 0x3);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      tc_commit_pair(drain);
+      volatile int no_abort = 0;
+      if (!mbar_wait(drain, 0, p.timeout_ns, &no_abort)) atomicOr(p.status, kErrTeardownWait);
+    }
+    grid_launch_dependents();
+  } else {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int q = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int i = pair; i < tiles; i += pairs) {
+      int ct, tt;
+      pair_tile(i, p, ct, tt);
+      const int t0 = tt * 256;
+      const Epi epi(args, ct * 256 + static_cast<int>(rank) * 128 + q * 32 + lane, p.channels);
+      const bool waited = mbar_wait(&tfull[acc], acc_phase, p.timeout_ns, abort_flag);
+      if (!__all_sync(0xffffffffu, waited)) {
+        if (lane == 0) fail(kErrEpilogueWait);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256);
+#pragma unroll 1
+      for (int b = 0; b < 8; ++b) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(t_row + b * 32, v);
+        tmem_ld_wait();
+        if (b == 7) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+        }
+        if (t0 + b * 32 < p.tokens) put32(epi, args, v, t0 + b * 32, p.tokens, lane);
+      }
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+  }
+  // Neither CTA releases TMEM or exits while its peer may still address it.
+  __syncwarp();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+}  // namespace pf

@@ -12,9 +12,9 @@
 #include <mutex>
 
 #include "pf_b200.h"
-#include "gemm8_simple.cuh"
+#include "gemm8_tc.cuh"
 #include "host_util.cuh"
-#include "quant_s8.cuh"
+#include "ops8_epilogue.cuh"
 
 // Bounded waits that ran out, of every kernel here: bits are only ever set, until pf_ops8_status clears them, so calls
 // that overlap on the GPU may share it.
@@ -28,11 +28,19 @@ typedef __nv_bfloat16 bf16;
 constexpr int kMaxDevices = 64;
 constexpr int kMaxSumK = 131071;  // K * 128 * 128 stays below 2^31
 
+// A device's properties and, for each tensor-core kernel that it has launched, the CTA pairs that fit at once (its
+// shared-memory limit raised before).
+struct KernelUnits {
+  const void *func;
+  int units;
+};
 struct Device {
   std::mutex mu;
   bool ready = false;
   int cc_major = 0, num_sms = 0;
   unsigned *status = nullptr;
+  KernelUnits kernels[48];
+  int n_kernels = 0;
 };
 Device g_devices[kMaxDevices];
 
@@ -133,9 +141,167 @@ struct BackwardSpace {
   }
 };
 
-template <class T, class Acc, class Store>
-void product(const pf::Strided<T> &g, int M, int N, int K, const Store &store, cudaStream_t s) {
-  pf::gemm8_simple<T, Acc><<<dim3(blocks_of(M, 64), blocks_of(N, 64)), 256, 0, s>>>(g, M, N, K, store);
+// TMA wants rows that start on 16-byte boundaries.  A product's operand that has others is copied, row by row, to the
+// workspace.
+struct ProductSpace {
+  bool copy_a, copy_b;
+  long long lda, ldb;  // row strides that the tensor maps use
+  size_t b, total;
+  static bool fits(const void *x, long long ld, int rows) { return pf::aligned16(x) && (rows == 1 || ld % 16 == 0); }
+  static long long round16(long long n) { return (n + 15) / 16 * 16; }
+  ProductSpace(int M, int N, int K, const void *A, long long lda_, const void *B, long long ldb_) {
+    copy_a = !fits(A, lda_, M);
+    copy_b = !fits(B, ldb_, K);
+    lda = copy_a || M == 1 ? round16(K) : lda_;
+    ldb = copy_b || K == 1 ? round16(N) : ldb_;
+    b = copy_a ? round256(size_t(M) * lda) : 0;
+    total = b + (copy_b ? round256(size_t(K) * ldb) : 0);
+  }
+};
+
+const void *aligned_copy(const signed char *X, long long ld, int rows, int cols, char *to, long long ld_to, cudaStream_t s) {
+  pf::align_rows<<<rows, 256, 0, s>>>(reinterpret_cast<const uint8_t *>(X), ld, cols, reinterpret_cast<uint4 *>(to), ld_to / 16);
+  return to;
+}
+
+// Raises a kernel's shared-memory limit and, for a pair kernel, counts the pairs that fit on the device at once.
+int kernel_units(Device &d, const void *func, int smem, int pair_threads, const Err &err, int *units) {
+  std::lock_guard<std::mutex> lk(d.mu);
+  for (int i = 0; i < d.n_kernels; ++i)
+    if (d.kernels[i].func == func) {
+      *units = d.kernels[i].units;
+      return PF_OK;
+    }
+  cudaError_t e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  int u = 0;
+  if (e == cudaSuccess && pair_threads) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(2 * (d.num_sms / 2));
+    cfg.blockDim = dim3(pair_threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&u, func, &cfg);
+    if (e == cudaSuccess && u <= 0) e = cudaErrorLaunchOutOfResources;
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return err(PF_ECUDA, "kernel set-up: %s", cudaGetErrorString(e));
+  }
+  if (d.n_kernels < static_cast<int>(sizeof d.kernels / sizeof d.kernels[0])) d.kernels[d.n_kernels++] = {func, u};
+  *units = u;
+  return PF_OK;
+}
+
+// One product: out[t][c] = sum_r T(t, r) W(r, c).  A K-major operand is [t][r] or [c][r], an MN-major one [r][t] or
+// [r][c], with row strides ldt, ldw in elements.
+struct Product {
+  int tokens, channels, sum;
+  const void *T, *W;
+  long long ldt, ldw;
+};
+
+template <int kElem>
+CUtensorMapDataType map_type() {
+  return kElem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+}
+
+template <class Op>
+int operand_maps(const Product &g, const Err &err, CUtensorMap *w, CUtensorMap *t) {
+  constexpr int e = Op::ELEM;
+  char msg[200];
+  if (pf::encode_2d_msg(msg, sizeof msg, w, map_type<e>(), g.W, Op::W_K ? g.sum : g.channels,
+                        Op::W_K ? g.channels : g.sum, g.ldw * e, Op::W_BOX0, Op::W_BOX1, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      pf::encode_2d_msg(msg, sizeof msg, t, map_type<e>(), g.T, Op::T_K ? g.sum : g.tokens, Op::T_K ? g.tokens : g.sum,
+                        g.ldt * e, Op::T_BOX0, Op::T_BOX1, CU_TENSOR_MAP_SWIZZLE_128B))
+    return err(PF_ECUDA, "%s", msg);
+  return PF_OK;
+}
+
+constexpr unsigned long long kWaitNs = 4000000000ull;
+constexpr int kSmemPerSm = 227 * 1024;  // of one SM, for the CTAs that share it
+
+template <class Op, class Epi>
+int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
+  CUtensorMap w, t;
+  int rc, units;
+  if ((rc = operand_maps<Op>(g, err, &w, &t))) return rc;
+  const void *func = reinterpret_cast<const void *>(&pf::gemm8_one<Op, Epi>);
+  if ((rc = kernel_units(d, func, kSmemPerSm - 1024, 0, err, &units))) return rc;
+  pf::Gemm8Params p = {};
+  p.channels = g.channels;
+  p.tokens = g.tokens;
+  p.c_tiles = (g.channels + 127) / 128;
+  p.t_tiles = (g.tokens + Op::TOKENS - 1) / Op::TOKENS;
+  p.k_blocks = (g.sum + Op::BK - 1) / Op::BK;
+  p.status = d.status;
+  p.timeout_ns = kWaitNs;
+  const long long tiles = static_cast<long long>(p.c_tiles) * p.t_tiles;
+  int splits = 1;
+  while (splits < 8 && tiles * splits < 2 * d.num_sms && p.k_blocks >= 4 * splits) splits *= 2;
+  // As deep a pipeline as lets the CTAs of one SM share its memory, at least what the split sums need.
+  const int per_sm = static_cast<int>(std::min<long long>(4, (tiles * splits + d.num_sms - 1) / d.num_sms));
+  const int room = (kSmemPerSm / per_sm - 1024 - 1024) / Op::STAGE_BYTES;
+  const int least = std::max(2, (Op::TOKENS * 512 + Op::STAGE_BYTES - 1) / Op::STAGE_BYTES);
+  p.stages = std::max(least, std::min({room, pf::kOneMaxStages, (p.k_blocks + splits - 1) / splits}));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.c_tiles * splits, p.t_tiles);
+  cfg.blockDim = dim3(pf::kOneThreads);
+  cfg.dynamicSmemBytes = 1024 + p.stages * Op::STAGE_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pf::pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, &pf::gemm8_one<Op, Epi>, w, t, p, args);
+  return launched(err);
+}
+
+template <class Op, class Epi, int kStages>
+int run_pair(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
+  using Cfg = pf::PairConfig<Op, kStages>;
+  CUtensorMap w, t;
+  int rc, units;
+  if ((rc = operand_maps<Op>(g, err, &w, &t))) return rc;
+  const void *func = reinterpret_cast<const void *>(&pf::gemm8_pair<Op, Epi, kStages>);
+  if ((rc = kernel_units(d, func, Cfg::SMEM_BYTES, Cfg::THREADS, err, &units))) return rc;
+  pf::Gemm8Params p = {};
+  p.channels = g.channels;
+  p.tokens = g.tokens;
+  p.c_tiles = (g.channels + 255) / 256;
+  p.t_tiles = (g.tokens + 255) / 256;
+  p.k_blocks = (g.sum + Op::BK - 1) / Op::BK;
+  p.group = std::min(16, p.c_tiles);
+  p.status = d.status;
+  p.timeout_ns = kWaitNs;
+  const long long tiles = static_cast<long long>(p.c_tiles) * p.t_tiles;
+  if (tiles > (1ll << 30)) return err(PF_EINVAL, "more than 2^30 tiles of 256 x 256");
+  pf::launch_pdl(&pf::gemm8_pair<Op, Epi, kStages>, dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, units))),
+                 Cfg::THREADS, Cfg::SMEM_BYTES, s, w, t, p, args);
+  return launched(err);
+}
+
+// Elements, W's and T's order, epilogue -> the kernel for the sizes.
+template <int kElem, bool kWK, bool kTK, class Epi>
+int product(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
+  using pf::Operands;
+  const long long pair_tiles = ((g.channels + 255ll) / 256) * ((g.tokens + 255ll) / 256);
+  if (g.tokens > 128 && pair_tiles >= 32)
+    return run_pair<Operands<kElem, kWK, kTK, 128, 2>, Epi, 3>(d, g, args, s, err);
+  if constexpr (kTK) {
+    if (g.tokens <= 16) return run_one<Operands<kElem, kWK, kTK, 16, 1>, Epi>(d, g, args, s, err);
+    if (g.tokens <= 32) return run_one<Operands<kElem, kWK, kTK, 32, 1>, Epi>(d, g, args, s, err);
+  }
+  if (g.tokens <= 64) return run_one<Operands<kElem, kWK, kTK, 64, 1>, Epi>(d, g, args, s, err);
+  return run_one<Operands<kElem, kWK, kTK, 128, 1>, Epi>(d, g, args, s, err);
 }
 
 }  // namespace
@@ -186,9 +352,14 @@ int pf_dequantize_s8(int device, int rows, int cols, const signed char *codes, l
   return launched(err);
 }
 
+size_t pf_gemm_s8_workspace(int M, int N, int K, const signed char *A, long long lda, const signed char *B,
+                            long long ldb) {
+  return M < 1 || N < 1 || K < 1 ? 0 : ProductSpace(M, N, K, A, lda, B, ldb).total;
+}
+
 int pf_gemm_s8(int device, int M, int N, int K, const signed char *A, long long lda, const signed char *B, long long ldb,
                const float *scale_a, const float *scale_b, const float *bias, int gelu, pf_dtype out, void *C,
-               long long ldc, void *stream, char *err_text, size_t err_len) {
+               long long ldc, void *workspace, size_t workspace_bytes, void *stream, char *err_text, size_t err_len) {
   const Err err{err_text, err_len};
   if (err_text && err_len) err_text[0] = '\0';
   if (M < 0 || N < 0) return err(PF_EINVAL, "M and N must not be negative (got %d, %d)", M, N);
@@ -196,17 +367,29 @@ int pf_gemm_s8(int device, int M, int N, int K, const signed char *A, long long 
     return err(PF_EINVAL, "K must be 1 to %d, so that a sum of int8 products fits 32 bits (got %d)", kMaxSumK, K);
   if (out != PF_F32 && out != PF_BF16) return err(PF_EINVAL, "the output type must be f32 or bf16");
   if (M == 0 || N == 0) return PF_OK;
-  if (any_null(A, B, C) || any_null(scale_a, scale_b)) return err(PF_EINVAL, "null argument");
+  if (any_null(A, B) || any_null(scale_a, scale_b) || any_null(C)) return err(PF_EINVAL, "null argument");
   if (lda < K || ldb < N || ldc < N) return err(PF_EINVAL, "a row stride is below the row's length");
+  const ProductSpace w(M, N, K, A, lda, B, ldb);
+  if (w.total && (!workspace || workspace_bytes < w.total))
+    return err(PF_EINVAL, "the workspace holds %zu bytes, %zu are needed", workspace ? workspace_bytes : size_t(0), w.total);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return err(PF_EINVAL, "the workspace must be 256-byte aligned");
   Device *d;
   cudaStream_t s;
   int rc;
   if ((rc = device_of(device, err, &d))) return rc;
   DeviceGuard g(device);
   if ((rc = stream_of(device, stream, err, &s))) return rc;
-  const pf::Strided<int8_t> op{reinterpret_cast<const int8_t *>(A), reinterpret_cast<const int8_t *>(B), lda, 1, ldb, 1};
-  product<int8_t, int>(op, M, N, K, pf::StoreS8{scale_a, scale_b, bias, gelu, out == PF_F32, C, ldc}, s);
-  return launched(err);
+  Product p{M, N, K, A, B, lda, ldb};
+  char *base = static_cast<char *>(workspace);
+  if (w.copy_a) p.T = aligned_copy(A, lda, M, K, base, w.lda, s);
+  if (w.copy_b) p.W = aligned_copy(B, ldb, K, N, base + w.b, w.ldb, s);
+  p.ldt = w.lda;
+  p.ldw = w.ldb;
+  if (out == PF_F32)
+    return product<1, false, true, pf::EpilogueS8<float>>(
+        *d, p, {scale_a, scale_b, bias, static_cast<float *>(C), ldc, gelu}, s, err);
+  return product<1, false, true, pf::EpilogueS8<bf16>>(*d, p, {scale_a, scale_b, bias, static_cast<bf16 *>(C), ldc, gelu},
+                                                       s, err);
 }
 
 int pf_gemm_bias_gelu_checkpoint(int device, int M, int N, int K, const void *A, const void *B, const float *bias,
@@ -228,9 +411,8 @@ int pf_gemm_bias_gelu_checkpoint(int device, int M, int N, int K, const void *A,
   DeviceGuard g(device);
   if ((rc = stream_of(device, stream, err, &s))) return rc;
   if (a_codes) quantize<bf16>(A, K, M, K, 1, reinterpret_cast<int8_t *>(a_codes), K, a_scale, s);
-  const pf::Strided<bf16> op{static_cast<const bf16 *>(A), static_cast<const bf16 *>(B), K, 1, N, 1};
-  product<bf16, float>(op, M, N, K, pf::StoreCheckpoint{bias, static_cast<bf16 *>(C), grad_codes, N}, s);
-  return launched(err);
+  return product<2, false, true, pf::EpilogueCheckpoint>(*d, Product{M, N, K, A, B, K, N},
+                                                         {bias, static_cast<bf16 *>(C), grad_codes, N}, s, err);
 }
 
 size_t pf_gemm_bias_gelu_backward_workspace(int M, int N, int K) {
@@ -270,14 +452,14 @@ int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, 
   pf::gelu_backward_dz<<<dim3(blocks_of(N, 256), w.parts), 256, 0, s>>>(
       static_cast<const bf16 *>(dC), grad_codes, dB ? a_scale : nullptr, M, N, dz, partial);
   if (dbias) pf::sum_partials<<<blocks_of(N, 256), 256, 0, s>>>(partial, w.parts, N, dbias);
-  if (dA) {
-    const pf::Strided<bf16> op{dz, static_cast<const bf16 *>(B), N, 1, 1, N};
-    product<bf16, float>(op, M, K, N, pf::StoreBf16{dB ? a_scale : nullptr, static_cast<bf16 *>(dA), K}, s);
-  }
+  if (dA && (rc = product<2, true, true, pf::EpilogueBf16>(*d, Product{M, K, N, dz, B, N, N},
+                                                           {dB ? a_scale : nullptr, static_cast<bf16 *>(dA), K}, s, err)))
+    return rc;
   if (dB) {
     pf::input_of_codes<<<M, 256, 0, s>>>(reinterpret_cast<const int8_t *>(a_codes), a_scale, K, a);
-    const pf::Strided<bf16> op{a, dz, 1, K, N, 1};
-    product<bf16, float>(op, K, N, M, pf::StoreBf16{nullptr, static_cast<bf16 *>(dB), N}, s);
+    if ((rc = product<2, false, false, pf::EpilogueBf16>(*d, Product{K, N, M, a, dz, K, N},
+                                                         {nullptr, static_cast<bf16 *>(dB), N}, s, err)))
+      return rc;
   }
   return launched(err);
 }

@@ -127,6 +127,24 @@ __global__ void dequantize_grad(const uint8_t *D, long long n, T *X) {
     X[i] = from_f32<T>(grad_value(D[i]));
 }
 
+// Rows of bytes that start anywhere -> rows of whole 16-byte words.  Each word is put together from the aligned
+// 4-byte words that hold its bytes; a word with no byte of the row is not read.  What follows a row's end is whatever
+// shares its last word, and is never used.
+__global__ void align_rows(const uint8_t *X, long long ld, int cols, uint4 *Y, long long ld_y) {
+  const long long r = blockIdx.x;
+  const uintptr_t row = reinterpret_cast<uintptr_t>(X + r * ld);
+  const unsigned shift = 8 * static_cast<unsigned>(row & 3);
+  const uint32_t *x = reinterpret_cast<const uint32_t *>(row & ~uintptr_t(3));
+  const int words = static_cast<int>((cols + (row & 3) + 3) / 4);
+  for (int i = threadIdx.x; i * 16 < cols; i += blockDim.x) {
+    uint32_t v[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) v[j] = i * 4 + j < words ? __ldg(x + i * 4 + j) : 0u;
+    Y[r * ld_y + i] = make_uint4(__funnelshift_r(v[0], v[1], shift), __funnelshift_r(v[1], v[2], shift),
+                                 __funnelshift_r(v[2], v[3], shift), __funnelshift_r(v[3], v[4], shift));
+  }
+}
+
 // The input's scale split into s = m 2^e, so that the backward pass rounds once where it could round twice: the
 // tensor cores take q 2^e, which is exact in bf16 (7 bits), and round(m dz), whose product is q s dz; dA, which
 // has no use for m, is divided by it at the end.  1 <= m < 2, so a token of tiny or no input keeps its dA.  A scale

@@ -161,8 +161,14 @@ def gemm_s8(A, B, scale_a, scale_b, bias=None, C=None, *, gelu: bool = False, dt
         with here:
             C = torch.empty((M, N), dtype=dtype, device=A.device)
     ldc = _matrix(C, "C", dtype, (M, N), A.device)[2]
-    _call("pf_gemm_s8", A.device.index, M, N, K, A.data_ptr(), lda, B.data_ptr(), ldb, scale_a.data_ptr(),
-          scale_b.data_ptr(), None if bias is None else bias.data_ptr(), int(gelu), out, C.data_ptr(), ldc, handle)
+    a, b, space = A.data_ptr(), B.data_ptr(), None
+    size = _pf.load_library().pf_gemm_s8_workspace(M, N, K, a, lda, b, ldb)  # 0 where rows start on 16-byte boundaries
+    if size:
+        with here:
+            space = torch.empty(size, dtype=torch.uint8, device=A.device)  # back to the stream's pool on return
+    _call("pf_gemm_s8", A.device.index, M, N, K, a, lda, b, ldb, scale_a.data_ptr(), scale_b.data_ptr(),
+          None if bias is None else bias.data_ptr(), int(gelu), out, C.data_ptr(), ldc,
+          None if space is None else space.data_ptr(), size, handle)
     return C
 
 

@@ -27,7 +27,11 @@ def dequantize(rows=4, cols=8, q=P, ldq=8, s=P, axis=1, dst=2, x=P, ldx=8):
 
 
 def gemm(M=4, N=8, K=16, a=P, lda=16, b=P, ldb=8, sa=P, sb=P, bias=None, out=2, c=P, ldc=8):
-    return call("pf_gemm_s8", 0, M, N, K, a, LL(lda), b, LL(ldb), sa, sb, bias, 0, out, c, LL(ldc), None)
+    return call("pf_gemm_s8", 0, M, N, K, a, LL(lda), b, LL(ldb), sa, sb, bias, 0, out, c, LL(ldc), None, 0, None)
+
+
+def unaligned():
+    return call("pf_gemm_s8", 0, 4, 8, 16, P, LL(17), P, LL(16), P, P, None, 0, 2, P, LL(8), P, 100, None)
 
 
 def forward(M=4, N=8, K=16, a=P, b=P, bias=P, c=P, q=P, s=P, d=P):
@@ -55,6 +59,8 @@ def forward(M=4, N=8, K=16, a=P, b=P, bias=P, c=P, q=P, s=P, d=P):
     (lambda: gemm(ldb=7), pf.PF_EINVAL, "stride"),
     (lambda: gemm(ldc=7), pf.PF_EINVAL, "stride"),
     (lambda: gemm(sb=None), pf.PF_EINVAL, "null"),
+    (lambda: gemm(), pf.PF_EINVAL, "workspace"),         # rows of B are 8 bytes
+    (lambda: unaligned(), pf.PF_EINVAL, "workspace holds 100 bytes"),
     (lambda: forward(N=0), pf.PF_EINVAL, "positive"),
     (lambda: forward(N=12), pf.PF_ESHAPE, "16 bytes"),
     (lambda: forward(K=20), pf.PF_ESHAPE, "16 bytes"),
@@ -79,10 +85,21 @@ def test_without_a_gpu_every_call_reports_it():
     if torch.cuda.is_available():
         pytest.skip("a GPU is visible")
     word = ctypes.c_uint()
-    for rc, _ in (quantize(), dequantize(), gemm(), forward(), call("pf_ops8_status", 0, ctypes.byref(word)),
+    for rc, _ in (quantize(), dequantize(), gemm(ldb=16), forward(), call("pf_ops8_status", 0, ctypes.byref(word)),
                   call("pf_dequantize_gelu_grad", 0, LL(1), P, 2, P, None),
                   call("pf_gemm_bias_gelu_backward", 0, 4, 8, 16, P, P, P, P, P, P, P, P, P, 1 << 20, None)):
         assert rc == pf.PF_ENODEV
+
+
+def test_product_workspace():
+    size = pf.load_library().pf_gemm_s8_workspace
+    args = lambda M, N, K, a, lda, b, ldb: (M, N, K, a, LL(lda), b, LL(ldb))  # noqa: E731
+    assert size(*args(4, 32, 16, P, 16, P, 32)) == 0
+    assert size(*args(1, 32, 17, P, 17, P, 32)) == 0                 # one row has no stride
+    assert size(*args(4, 32, 17, P, 17, P, 32)) == 256               # A: 4 rows of 32 bytes
+    assert size(*args(4, 33, 16, P, 16, P, 33)) == 768               # B: 16 rows of 48 bytes
+    assert size(*args(4, 33, 17, P + 1, 32, P, 33)) == 256 + 1024    # both; B: 17 rows of 48 bytes
+    assert size(*args(1 << 20, 32, 100001, P, 100001, P, 32)) >= (1 << 20) * 100001  # past 32 bits
 
 
 def test_backward_workspace():
