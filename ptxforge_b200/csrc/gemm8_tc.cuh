@@ -86,6 +86,7 @@ struct EpilogueS8 {
     long long ld;
     int gelu;
   };
+  static constexpr bool kTokenScalar = true;
   const Args &a;
   const int c;
   const bool inside;
@@ -97,10 +98,32 @@ struct EpilogueS8 {
   }
   static __device__ __forceinline__ float token(const Args &a, int t) { return __ldg(a.sa + t); }
   static __device__ __forceinline__ uint32_t add(uint32_t x, uint32_t y) { return x + y; }
+  // Two tokens' sums and scalars -> their values.
+  template <bool kGelu>
+  __device__ __forceinline__ float2 value(uint32_t s0, uint32_t s1, float a0, float a1) const {
+    const float2 x = __ffma2_rn(make_float2(static_cast<float>(static_cast<int>(s0)), static_cast<float>(static_cast<int>(s1))),
+                                __fmul2_rn(make_float2(a0, a1), both(sb)), both(bias));
+    return kGelu ? gelu_of(x) : x;
+  }
   __device__ __forceinline__ void put(uint32_t sum, int t, float sa) const {
-    float x = fmaf(static_cast<float>(static_cast<int>(sum)), sa * sb, bias);
-    if (a.gelu) x = gelu_of(x);
-    if (inside) a.out[t * a.ld + c] = from_f32<Out>(x);
+    const float2 y = a.gelu ? value<true>(sum, sum, sa, sa) : value<false>(sum, sum, sa, sa);
+    if (inside) a.out[t * a.ld + c] = from_f32<Out>(y.x);
+  }
+  template <bool kGelu>
+  __device__ __forceinline__ void put32_as(const uint32_t (&v)[32], int t0, const float *scalars) const {
+    Out *out = a.out + t0 * a.ld + c;
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float2 y = value<kGelu>(v[j], v[j + 1], scalars[j], scalars[j + 1]);
+      if (inside) {
+        out[j * a.ld] = from_f32<Out>(y.x);
+        out[(j + 1) * a.ld] = from_f32<Out>(y.y);
+      }
+    }
+  }
+  __device__ __forceinline__ void put32(const uint32_t (&v)[32], int t0, const float *scalars) const {
+    if (a.gelu) put32_as<true>(v, t0, scalars);
+    else put32_as<false>(v, t0, scalars);
   }
 };
 
@@ -117,6 +140,7 @@ struct EpilogueCheckpoint : EpilogueF32Sum {
     uint8_t *codes;
     long long ld;
   };
+  static constexpr bool kTokenScalar = false;
   const Args &a;
   const int c;
   const bool inside;
@@ -127,42 +151,85 @@ struct EpilogueCheckpoint : EpilogueF32Sum {
   }
   static __device__ __forceinline__ float token(const Args &, int) { return 0.f; }
   __device__ __forceinline__ void put(uint32_t sum, int t, float) const {
-    const Gelu g = gelu_and_grad(__uint_as_float(sum) + bias);
+    const float x = __uint_as_float(sum) + bias;
+    const Gelu2 g = gelu_and_grad(make_float2(x, x));
     if (inside) {
-      a.out[t * a.ld + c] = __float2bfloat16_rn(g.y);
-      a.codes[t * a.ld + c] = static_cast<uint8_t>(grad_code(g.d));
+      a.out[t * a.ld + c] = __float2bfloat16_rn(g.y.x);
+      a.codes[t * a.ld + c] = static_cast<uint8_t>(grad_codes(g.d).x);
+    }
+  }
+  __device__ __forceinline__ void put32(const uint32_t (&v)[32], int t0, const float *) const {
+    const long long i = t0 * a.ld + c;
+    __nv_bfloat16 *out = a.out + i;
+    uint8_t *codes = a.codes + i;
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const Gelu2 g = gelu_and_grad(__fadd2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), both(bias)));
+      const uint2 code = grad_codes(g.d);
+      if (inside) {
+        out[j * a.ld] = __float2bfloat16_rn(g.y.x);
+        out[(j + 1) * a.ld] = __float2bfloat16_rn(g.y.y);
+        codes[j * a.ld] = static_cast<uint8_t>(code.x);
+        codes[(j + 1) * a.ld] = static_cast<uint8_t>(code.y);
+      }
     }
   }
 };
 
+// kDivided: a token's row is divided by its m (split_scale of its input scale).
+template <bool kDivided>
 struct EpilogueBf16 : EpilogueF32Sum {
   struct Args {
-    const float *token_scale;  // null, or a token's row is divided by its m (split_scale)
+    const float *token_scale;
     __nv_bfloat16 *out;
     long long ld;
   };
+  static constexpr bool kTokenScalar = kDivided;
   const Args &a;
   const int c;
   const bool inside;
   __device__ __forceinline__ EpilogueBf16(const Args &args, int channel, int channels)
       : a(args), c(channel), inside(channel < channels) {}
   static __device__ __forceinline__ float token(const Args &a, int t) {
-    return a.token_scale ? __fdiv_rn(1.f, split_scale(__ldg(a.token_scale + t)).m) : 1.f;
+    return kDivided ? __fdiv_rn(1.f, split_scale(__ldg(a.token_scale + t)).m) : 1.f;
   }
   __device__ __forceinline__ void put(uint32_t sum, int t, float inv_m) const {
     if (inside) a.out[t * a.ld + c] = __float2bfloat16_rn(__uint_as_float(sum) * inv_m);
   }
+  __device__ __forceinline__ void put32(const uint32_t (&v)[32], int t0, const float *scalars) const {
+    __nv_bfloat16 *out = a.out + t0 * a.ld + c;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const __nv_bfloat16 y = __float2bfloat16_rn(__uint_as_float(v[j]) * (kDivided ? scalars[j] : 1.f));
+      if (inside) out[j * a.ld] = y;
+    }
+  }
 };
 
-// 32 tokens from t0 on: lane j holds token t0 + j's scalar.
+// The scalars of tokens [t0, t0 + 32 n) into this warp's shared memory, from which a broadcast load brings four.
 template <class Epi>
-__device__ __forceinline__ void put32(const Epi &e, const typename Epi::Args &args, const uint32_t (&v)[32], int t0,
-                                      int tokens, int lane) {
-  const float mine = t0 + lane < tokens ? Epi::token(args, t0 + lane) : 0.f;
+__device__ __forceinline__ void stage_scalars(const typename Epi::Args &args, int t0, int n, int tokens, int lane,
+                                              float *scalars) {
+  if constexpr (Epi::kTokenScalar) {
+    __syncwarp();  // the last tile's were read
+    for (int b = 0; b < n; ++b) {
+      const int t = t0 + b * 32 + lane;
+      scalars[b * 32 + lane] = t < tokens ? Epi::token(args, t) : 0.f;
+    }
+    __syncwarp();
+  }
+}
+
+// 32 tokens from t0 on.  Whole blocks run without a branch a token, so that the arithmetic of many overlaps (with one, a
+// tile of 256 x 256 took 27 us).
+template <class Epi>
+__device__ __forceinline__ void put32(const Epi &e, const uint32_t (&v)[32], int t0, int tokens, const float *scalars) {
+  if (t0 + 32 <= tokens) {
+    e.put32(v, t0, scalars);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float s = __shfl_sync(0xffffffffu, mine, j);
-    if (t0 + j < tokens) e.put(v[j], t0 + j, s);
+    for (int j = 0; j < 32; ++j)
+      if (t0 + j < tokens) e.put(v[j], t0 + j, Epi::kTokenScalar ? scalars[j] : 0.f);
   }
 }
 
@@ -190,6 +257,7 @@ __global__ void __launch_bounds__(kOneThreads)
   __shared__ uint64_t full[kOneMaxStages], empty[kOneMaxStages], done;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_word;
+  __shared__ __align__(16) float scalars[4][TOKENS < 32 ? 32 : TOKENS];
   volatile int *abort_flag = &abort_word;
   uint8_t *sW = smem, *sT = smem + p.stages * Op::W_BYTES;
 
@@ -297,6 +365,7 @@ __global__ void __launch_bounds__(kOneThreads)
     const int c_local = q * 32 + lane;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const Epi epi(args, c0 + c_local, p.channels);
+    if (splits == 1) stage_scalars<Epi>(args, t0, (TOKENS + 31) / 32, p.tokens, lane, scalars[q]);
     const bool waited = mbar_wait(&done, 0, p.timeout_ns, abort_flag);
     if (!__all_sync(0xffffffffu, waited)) {
       if (lane == 0) fail(kErrEpilogueWait);
@@ -310,7 +379,7 @@ __global__ void __launch_bounds__(kOneThreads)
         tmem_ld_32x32b_x32(t_row + b * 32, v);
         tmem_ld_wait();
         if (splits == 1) {
-          put32(epi, args, v, t0 + b * 32, min(p.tokens, t0 + TOKENS), lane);
+          put32(epi, v, t0 + b * 32, min(p.tokens, t0 + TOKENS), scalars[q] + b * 32);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
@@ -361,7 +430,8 @@ __device__ __forceinline__ void pair_tile(int i, const Gemm8Params &p, int &ct, 
 template <class Op, int kStages>
 struct PairConfig {
   static constexpr int STAGES = kStages;
-  static constexpr int EPI_WARPS = 4;
+  static constexpr int EPI_WARPS = 8;    // two to a quarter of the TMEM lanes, each with half of the tokens
+  static constexpr int EPI_BLOCKS = 4;   // blocks of 32 tokens a warp
   static constexpr int THREADS = 64 + EPI_WARPS * 32;
   static constexpr int NUM_BARS = 2 * STAGES + 4 + 1;
   static constexpr int SMEM_BYTES = 1024 + STAGES * Op::STAGE_BYTES + NUM_BARS * 8 + 16;
@@ -375,6 +445,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
     gemm8_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const Gemm8Params p,
                const typename Epi::Args args) {
   using Cfg = PairConfig<Op, kStages>;
+  __shared__ __align__(16) float scalars[Cfg::EPI_WARPS][Cfg::EPI_BLOCKS * 32];
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sW = smem, *sT = smem + Cfg::STAGES * Op::W_BYTES;
@@ -513,32 +584,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
   } else {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int q = warp & 3;
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    float *mine = scalars[warp - 2];
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int i = pair; i < tiles; i += pairs) {
       int ct, tt;
       pair_tile(i, p, ct, tt);
-      const int t0 = tt * 256;
+      const int t0 = tt * 256 + half * 128;
+      // what belongs to the channel and the tokens is loaded while the accumulator fills
       const Epi epi(args, ct * 256 + static_cast<int>(rank) * 128 + q * 32 + lane, p.channels);
+      stage_scalars<Epi>(args, t0, Cfg::EPI_BLOCKS, p.tokens, lane, mine);
       const bool waited = mbar_wait(&tfull[acc], acc_phase, p.timeout_ns, abort_flag);
       if (!__all_sync(0xffffffffu, waited)) {
         if (lane == 0) fail(kErrEpilogueWait);
         break;
       }
       tc_fence_after();
-      const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256);
-#pragma unroll 1
-      for (int b = 0; b < 8; ++b) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(t_row + b * 32, v);
+      const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256 + half * 128);
+      // The next block's sums travel from TMEM while this block's values are computed.
+      uint32_t v[2][32];
+      tmem_ld_32x32b_x32(t_row, v[0]);
+#pragma unroll
+      for (int b = 0; b < Cfg::EPI_BLOCKS; ++b) {
         tmem_ld_wait();
-        if (b == 7) {
+        if (b + 1 < Cfg::EPI_BLOCKS) {
+          tmem_ld_32x32b_x32(t_row + (b + 1) * 32, v[(b + 1) & 1]);
+        } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
         }
-        if (t0 + b * 32 < p.tokens) put32(epi, args, v, t0 + b * 32, p.tokens, lane);
+        if (t0 + b * 32 < p.tokens) put32(epi, v[b & 1], t0 + b * 32, p.tokens, mine + b * 32);
       }
       if (++acc == 2) {
         acc = 0;

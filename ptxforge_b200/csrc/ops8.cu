@@ -452,12 +452,16 @@ int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, 
   pf::gelu_backward_dz<<<dim3(blocks_of(N, 256), w.parts), 256, 0, s>>>(
       static_cast<const bf16 *>(dC), grad_codes, dB ? a_scale : nullptr, M, N, dz, partial);
   if (dbias) pf::sum_partials<<<blocks_of(N, 256), 256, 0, s>>>(partial, w.parts, N, dbias);
-  if (dA && (rc = product<2, true, true, pf::EpilogueBf16>(*d, Product{M, K, N, dz, B, N, N},
-                                                           {dB ? a_scale : nullptr, static_cast<bf16 *>(dA), K}, s, err)))
-    return rc;
+  if (dA) {
+    const Product g{M, K, N, dz, B, N, N};
+    bf16 *out = static_cast<bf16 *>(dA);
+    rc = dB ? product<2, true, true, pf::EpilogueBf16<true>>(*d, g, {a_scale, out, K}, s, err)
+            : product<2, true, true, pf::EpilogueBf16<false>>(*d, g, {nullptr, out, K}, s, err);
+    if (rc) return rc;
+  }
   if (dB) {
     pf::input_of_codes<<<M, 256, 0, s>>>(reinterpret_cast<const int8_t *>(a_codes), a_scale, K, a);
-    if ((rc = product<2, false, false, pf::EpilogueBf16>(*d, Product{K, N, M, a, dz, K, N},
+    if ((rc = product<2, false, false, pf::EpilogueBf16<false>>(*d, Product{K, N, M, a, dz, K, N},
                                                          {nullptr, static_cast<bf16 *>(dB), N}, s, err)))
       return rc;
   }

@@ -55,10 +55,6 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
   return max(-127, min(127, q));
 }
 
-__device__ __forceinline__ uint32_t grad_code(float d) {
-  if (d != d) return kGradNan;
-  return static_cast<uint32_t>(__float2int_rn(d * kGradSteps) + kGradZero);
-}
 __device__ __forceinline__ float grad_value(uint32_t code) {
   const float d = __fdiv_rn(static_cast<float>(static_cast<int>(code) - kGradZero), kGradSteps);
   return code == kGradNan ? __uint_as_float(0x7FC00000u) : d;

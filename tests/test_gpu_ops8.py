@@ -201,7 +201,7 @@ def test_product_of_a_token_with_a_nan_scale_is_nan_there_alone():
 # the product with an 8-bit checkpoint, and its gradients
 # ---------------------------------------------------------------------------------------------
 LAYERS = [(1, 8, 8), (1, 136, 72), (7, 64, 256), (77, 512, 512), (128, 128, 64), (129, 264, 136), (200, 136, 72),
-          (256, 256, 256), (300, 1024, 520), (515, 776, 1032), (1000, 72, 2048), (2100, 2056, 264)]
+          (256, 256, 256), (300, 1024, 520), (515, 776, 1032), (1000, 72, 2048), (2100, 2056, 264), (1601, 1544, 1288)]
 
 
 def layer(M, N, K, seed=0):
