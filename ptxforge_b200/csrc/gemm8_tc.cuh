@@ -194,7 +194,7 @@ struct EpilogueBf16 : EpilogueF32Sum {
     return kDivided ? __fdiv_rn(1.f, split_scale(__ldg(a.token_scale + t)).m) : 1.f;
   }
   __device__ __forceinline__ void put(uint32_t sum, int t, float inv_m) const {
-    if (inside) a.out[t * a.ld + c] = __float2bfloat16_rn(__uint_as_float(sum) * inv_m);
+    if (inside) a.out[t * a.ld + c] = __float2bfloat16_rn(__uint_as_float(sum) * (kDivided ? inv_m : 1.f));
   }
   __device__ __forceinline__ void put32(const uint32_t (&v)[32], int t0, const float *scalars) const {
     __nv_bfloat16 *out = a.out + t0 * a.ld + c;

@@ -224,6 +224,7 @@ int operand_maps(const Product &g, const Err &err, CUtensorMap *w, CUtensorMap *
 
 constexpr unsigned long long kWaitNs = 4000000000ull;
 constexpr int kSmemPerSm = 227 * 1024;  // of one SM, for the CTAs that share it
+constexpr int kOneStatic = 3072;        // of gemm8_one: barriers and token scalars
 
 template <class Op, class Epi>
 int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
@@ -231,7 +232,7 @@ int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStr
   int rc, units;
   if ((rc = operand_maps<Op>(g, err, &w, &t))) return rc;
   const void *func = reinterpret_cast<const void *>(&pf::gemm8_one<Op, Epi>);
-  if ((rc = kernel_units(d, func, kSmemPerSm - 1024, 0, err, &units))) return rc;
+  if ((rc = kernel_units(d, func, kSmemPerSm - kOneStatic, 0, err, &units))) return rc;
   pf::Gemm8Params p = {};
   p.channels = g.channels;
   p.tokens = g.tokens;
@@ -245,7 +246,7 @@ int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStr
   while (splits < 8 && tiles * splits < 2 * d.num_sms && p.k_blocks >= 4 * splits) splits *= 2;
   // As deep a pipeline as lets the CTAs of one SM share its memory, at least what the split sums need.
   const int per_sm = static_cast<int>(std::min<long long>(4, (tiles * splits + d.num_sms - 1) / d.num_sms));
-  const int room = (kSmemPerSm / per_sm - 1024 - 1024) / Op::STAGE_BYTES;
+  const int room = (kSmemPerSm / per_sm - kOneStatic - 2048) / Op::STAGE_BYTES;  // alignment, and 1 KB of the system's
   const int least = std::max(2, (Op::TOKENS * 512 + Op::STAGE_BYTES - 1) / Op::STAGE_BYTES);
   p.stages = std::max(least, std::min({room, pf::kOneMaxStages, (p.k_blocks + splits - 1) / splits}));
   cudaLaunchConfig_t cfg = {};
