@@ -239,12 +239,6 @@ __device__ __forceinline__ void put32(const Epi &e, const uint32_t (&v)[32], int
 constexpr int kOneThreads = 192;
 constexpr int kOneMaxStages = 16;
 
-__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 template <class Op, class Epi>
 __global__ void __launch_bounds__(kOneThreads)
     gemm8_one(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const Gemm8Params p,

@@ -29,22 +29,32 @@ inline bool pdl_enabled() {
   return on;
 }
 
+// A launch with clusters of `cluster` CTAs along x where that is above 0 (otherwise as the kernel says).
 template <class... Params, class... Args>
-void launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args &&...args) {
+void launch_cluster(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, int cluster, cudaStream_t s, Args &&...args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.numAttrs = 0;
   if (pdl_enabled()) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 0) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
   }
   cfg.attrs = attr;
   cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);  // errors surface through cudaGetLastError
+}
+template <class... Params, class... Args>
+void launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStream_t s, Args &&...args) {
+  launch_cluster(kernel, grid, block, smem, 0, s, std::forward<Args>(args)...);
 }
 
 // The driver's cuTensorMapEncodeTiled.  A function-local static is initialised exactly once, and threads

@@ -114,16 +114,114 @@ bool any_null(const P *...p) {
 
 unsigned blocks_of(long long n, int per) { return static_cast<unsigned>((n + per - 1) / per); }
 
-template <class T>
-void quantize(const void *X, long long ldx, int rows, int cols, int axis, int8_t *Q, long long ldq, float *scale,
-              cudaStream_t s) {
-  const T *x = static_cast<const T *>(X);
-  if (axis == 1) {
-    pf::quantize_rows_s8<T><<<rows, 256, 0, s>>>(x, ldx, cols, Q, ldq, scale);
-  } else {
-    pf::scale_cols_s8<T><<<blocks_of(cols, 32), dim3(32, 8), 0, s>>>(x, ldx, rows, cols, scale);
-    pf::quantize_cols_s8<T><<<rows, 256, 0, s>>>(x, ldx, cols, scale, Q, ldq);
+// Raises a kernel's shared-memory limit and, for a pair kernel, counts the pairs that fit on the device at once.
+int kernel_units(Device &d, const void *func, int smem, int pair_threads, const Err &err, int *units) {
+  std::lock_guard<std::mutex> lk(d.mu);
+  for (int i = 0; i < d.n_kernels; ++i)
+    if (d.kernels[i].func == func) {
+      *units = d.kernels[i].units;
+      return PF_OK;
+    }
+  cudaError_t e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  int u = 0;
+  if (e == cudaSuccess && pair_threads) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(2 * (d.num_sms / 2));
+    cfg.blockDim = dim3(pair_threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&u, func, &cfg);
+    if (e == cudaSuccess && u <= 0) e = cudaErrorLaunchOutOfResources;
   }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return err(PF_ECUDA, "kernel set-up: %s", cudaGetErrorString(e));
+  }
+  if (d.n_kernels < static_cast<int>(sizeof d.kernels / sizeof d.kernels[0])) d.kernels[d.n_kernels++] = {func, u};
+  *units = u;
+  return PF_OK;
+}
+
+// Whether rows of `cols` values of `size` bytes, `ld` apart, can be read and written `vec` values at a time.
+bool vectors_fit(const void *x, long long ld, int cols, int size, int vec) {
+  return reinterpret_cast<uintptr_t>(x) % (size * vec) == 0 && ld % vec == 0 && cols % vec == 0;
+}
+
+template <class T, int kVec>
+void quantize_rows(const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale, cudaStream_t s) {
+  // A warp a row, several rows a block, where its registers hold the row; else a block a row, of as many threads as
+  // the row needs with as few vectors each as 256 threads allow (so that a lone row is spread over a whole SM).
+  const int vecs = (cols + kVec - 1) / kVec;
+  const auto launch = [&](auto kernel, dim3 block) {
+    pf::launch_pdl(kernel, dim3(blocks_of(rows, block.y)), block, 0, s, x, ldx, rows, cols, q, ldq, scale);
+  };
+  if (vecs <= 64) return launch(&pf::quantize_rows_s8<T, kVec, 2>, dim3(32, 8));
+  const auto threads = [&](int held) { return dim3(std::min(512, (vecs + 32 * held - 1) / (32 * held) * 32)); };
+  if (vecs <= 512) return launch(&pf::quantize_rows_s8<T, kVec, 2>, threads(2));
+  if (vecs <= 1024) return launch(&pf::quantize_rows_s8<T, kVec, 4>, threads(4));
+  launch(&pf::quantize_rows_s8<T, kVec, 8>, threads(8));
+}
+
+template <class T, int kVec>
+int quantize_cols(Device &d, const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale,
+                  cudaStream_t s, const Err &err) {
+  // 512 rows of 128 bytes a CTA (three CTAs share an SM, one's loads beside another's stores) as long as 8 CTAs take
+  // them all; above, what an SM's shared memory holds.
+  constexpr int kRowBytes = 128, kMostHeld = 220 * 1024 / kRowBytes;
+  int splits = 1;
+  while (splits < 8 && rows > 512 * splits) splits *= 2;
+  const int share = (rows + splits - 1) / splits, held = std::min(share, kMostHeld);
+  const void *func = reinterpret_cast<const void *>(&pf::quantize_cols_s8<T, kVec>);
+  int rc, units;
+  if ((rc = kernel_units(d, func, kMostHeld * kRowBytes, 0, err, &units))) return rc;
+  pf::launch_cluster(&pf::quantize_cols_s8<T, kVec>, dim3(blocks_of(static_cast<long long>(cols) * sizeof(T), kRowBytes) * splits),
+                     dim3(256), held * kRowBytes, splits, s, x, ldx, rows, cols, held, q, ldq, scale);
+  return PF_OK;
+}
+
+template <class T>
+int quantize(Device &d, const void *X, long long ldx, int rows, int cols, int axis, int8_t *Q, long long ldq, float *scale,
+             cudaStream_t s, const Err &err) {
+  constexpr int kVec = 16 / sizeof(T);
+  const T *x = static_cast<const T *>(X);
+  const bool wide = vectors_fit(X, ldx, cols, sizeof(T), kVec) && vectors_fit(Q, ldq, cols, 1, kVec);
+  if (axis == 0)
+    return wide ? quantize_cols<T, kVec>(d, x, ldx, rows, cols, Q, ldq, scale, s, err)
+                : quantize_cols<T, 1>(d, x, ldx, rows, cols, Q, ldq, scale, s, err);
+  if (wide) quantize_rows<T, kVec>(x, ldx, rows, cols, Q, ldq, scale, s);
+  else quantize_rows<T, 1>(x, ldx, rows, cols, Q, ldq, scale, s);
+  return PF_OK;
+}
+
+template <class T, int kVec>
+void dequantize(const int8_t *q, long long ldq, int rows, int cols, const float *scale, int axis, T *x, long long ldx,
+                cudaStream_t s) {
+  int across = 8;  // threads a row
+  while (across < 256 && across * kVec < cols) across *= 2;
+  const dim3 block(across, 256 / across);
+  const auto kernel = axis ? &pf::dequantize_s8<T, kVec, true> : &pf::dequantize_s8<T, kVec, false>;
+  pf::launch_pdl(kernel, dim3(blocks_of(rows, block.y)), block, 0, s, q, ldq, rows, cols, scale, x, ldx);
+}
+template <class T>
+void dequantize(const int8_t *q, long long ldq, int rows, int cols, const float *scale, int axis, void *X, long long ldx,
+                cudaStream_t s) {
+  T *x = static_cast<T *>(X);
+  if (vectors_fit(q, ldq, cols, 1, 8) && vectors_fit(X, ldx, cols, sizeof(T), 8)) dequantize<T, 8>(q, ldq, rows, cols, scale, axis, x, ldx, s);
+  else dequantize<T, 1>(q, ldq, rows, cols, scale, axis, x, ldx, s);
+}
+
+template <class T>
+void dequantize_grad(const unsigned char *codes, long long n, void *X, cudaStream_t s) {
+  T *x = static_cast<T *>(X);
+  const bool wide = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && pf::aligned16(X);
+  const int per = 256 * (wide ? 8 : 1);
+  const dim3 grid(static_cast<unsigned>(std::min<long long>((n + per - 1) / per, 1 << 30)));
+  pf::launch_pdl(wide ? &pf::dequantize_grad<T, 8> : &pf::dequantize_grad<T, 1>, grid, 256, 0, s, codes, n, x);
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -160,41 +258,9 @@ struct ProductSpace {
 };
 
 const void *aligned_copy(const signed char *X, long long ld, int rows, int cols, char *to, long long ld_to, cudaStream_t s) {
-  pf::align_rows<<<rows, 256, 0, s>>>(reinterpret_cast<const uint8_t *>(X), ld, cols, reinterpret_cast<uint4 *>(to), ld_to / 16);
+  pf::launch_pdl(&pf::align_rows, dim3(rows), 256, 0, s, reinterpret_cast<const uint8_t *>(X), ld, cols,
+                 reinterpret_cast<uint4 *>(to), ld_to / 16);
   return to;
-}
-
-// Raises a kernel's shared-memory limit and, for a pair kernel, counts the pairs that fit on the device at once.
-int kernel_units(Device &d, const void *func, int smem, int pair_threads, const Err &err, int *units) {
-  std::lock_guard<std::mutex> lk(d.mu);
-  for (int i = 0; i < d.n_kernels; ++i)
-    if (d.kernels[i].func == func) {
-      *units = d.kernels[i].units;
-      return PF_OK;
-    }
-  cudaError_t e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  int u = 0;
-  if (e == cudaSuccess && pair_threads) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(2 * (d.num_sms / 2));
-    cfg.blockDim = dim3(pair_threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaOccupancyMaxActiveClusters(&u, func, &cfg);
-    if (e == cudaSuccess && u <= 0) e = cudaErrorLaunchOutOfResources;
-  }
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return err(PF_ECUDA, "kernel set-up: %s", cudaGetErrorString(e));
-  }
-  if (d.n_kernels < static_cast<int>(sizeof d.kernels / sizeof d.kernels[0])) d.kernels[d.n_kernels++] = {func, u};
-  *units = u;
-  return PF_OK;
 }
 
 // One product: out[t][c] = sum_r T(t, r) W(r, c).  A K-major operand is [t][r] or [c][r], an MN-major one [r][t] or
@@ -249,20 +315,8 @@ int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStr
   const int room = (kSmemPerSm / per_sm - kOneStatic - 2048) / Op::STAGE_BYTES;  // alignment, and 1 KB of the system's
   const int least = std::max(2, (Op::TOKENS * 512 + Op::STAGE_BYTES - 1) / Op::STAGE_BYTES);
   p.stages = std::max(least, std::min({room, pf::kOneMaxStages, (p.k_blocks + splits - 1) / splits}));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.c_tiles * splits, p.t_tiles);
-  cfg.blockDim = dim3(pf::kOneThreads);
-  cfg.dynamicSmemBytes = 1024 + p.stages * Op::STAGE_BYTES;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pf::pdl_enabled() ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, &pf::gemm8_one<Op, Epi>, w, t, p, args);
+  pf::launch_cluster(&pf::gemm8_one<Op, Epi>, dim3(p.c_tiles * splits, p.t_tiles), dim3(pf::kOneThreads),
+                     1024 + p.stages * Op::STAGE_BYTES, splits, s, w, t, p, args);
   return launched(err);
 }
 
@@ -326,9 +380,9 @@ int pf_quantize_s8(int device, pf_dtype src, int rows, int cols, const void *X, 
   DeviceGuard g(device);
   if ((rc = stream_of(device, stream, err, &s))) return rc;
   int8_t *q = reinterpret_cast<int8_t *>(codes);
-  if (src == PF_F32) quantize<float>(X, ldx, rows, cols, axis, q, ld_codes, scale, s);
-  else quantize<bf16>(X, ldx, rows, cols, axis, q, ld_codes, scale, s);
-  return launched(err);
+  rc = src == PF_F32 ? quantize<float>(*d, X, ldx, rows, cols, axis, q, ld_codes, scale, s, err)
+                     : quantize<bf16>(*d, X, ldx, rows, cols, axis, q, ld_codes, scale, s, err);
+  return rc ? rc : launched(err);
 }
 
 int pf_dequantize_s8(int device, int rows, int cols, const signed char *codes, long long ld_codes, const float *scale,
@@ -348,8 +402,8 @@ int pf_dequantize_s8(int device, int rows, int cols, const signed char *codes, l
   DeviceGuard g(device);
   if ((rc = stream_of(device, stream, err, &s))) return rc;
   const int8_t *q = reinterpret_cast<const int8_t *>(codes);
-  if (dst == PF_F32) pf::dequantize_s8<float><<<rows, 256, 0, s>>>(q, ld_codes, cols, scale, axis, static_cast<float *>(X), ldx);
-  else pf::dequantize_s8<bf16><<<rows, 256, 0, s>>>(q, ld_codes, cols, scale, axis, static_cast<bf16 *>(X), ldx);
+  if (dst == PF_F32) dequantize<float>(q, ld_codes, rows, cols, scale, axis, X, ldx, s);
+  else dequantize<bf16>(q, ld_codes, rows, cols, scale, axis, X, ldx, s);
   return launched(err);
 }
 
@@ -411,7 +465,7 @@ int pf_gemm_bias_gelu_checkpoint(int device, int M, int N, int K, const void *A,
   if ((rc = device_of(device, err, &d))) return rc;
   DeviceGuard g(device);
   if ((rc = stream_of(device, stream, err, &s))) return rc;
-  if (a_codes) quantize<bf16>(A, K, M, K, 1, reinterpret_cast<int8_t *>(a_codes), K, a_scale, s);
+  if (a_codes && (rc = quantize<bf16>(*d, A, K, M, K, 1, reinterpret_cast<int8_t *>(a_codes), K, a_scale, s, err))) return rc;
   return product<2, false, true, pf::EpilogueCheckpoint>(*d, Product{M, N, K, A, B, K, N},
                                                          {bias, static_cast<bf16 *>(C), grad_codes, N}, s, err);
 }
@@ -450,9 +504,15 @@ int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, 
   char *base = static_cast<char *>(workspace);
   bf16 *dz = reinterpret_cast<bf16 *>(base + w.dz), *a = reinterpret_cast<bf16 *>(base + w.a);
   float *partial = reinterpret_cast<float *>(base + w.partial);
-  pf::gelu_backward_dz<<<dim3(blocks_of(N, 256), w.parts), 256, 0, s>>>(
-      static_cast<const bf16 *>(dC), grad_codes, dB ? a_scale : nullptr, M, N, dz, partial);
-  if (dbias) pf::sum_partials<<<blocks_of(N, 256), 256, 0, s>>>(partial, w.parts, N, dbias);
+  const int col_blocks = (N + pf::kDzCols - 1) / pf::kDzCols;
+  const long long dz_blocks = static_cast<long long>(col_blocks) * w.parts, blocks = dz_blocks + (dB ? M : 0);
+  if (blocks > 0x7FFFFFFF) return err(PF_EINVAL, "more than 2^31 blocks");
+  float *sums = dbias && w.parts == 1 ? dbias : partial;
+  pf::launch_pdl(&pf::backward_operands, dim3(static_cast<unsigned>(blocks)), 256, 0, s, static_cast<const bf16 *>(dC), grad_codes,
+                 dB ? a_scale : static_cast<const float *>(nullptr), M, N, static_cast<int>(dz_blocks), col_blocks, dz, sums,
+                 reinterpret_cast<const int8_t *>(a_codes), K, a);
+  if (dbias && w.parts > 1)
+    pf::launch_pdl(&pf::sum_row_blocks, dim3(blocks_of(N, 32)), 256, 0, s, static_cast<const float *>(partial), w.parts, N, dbias);
   if (dA) {
     const Product g{M, K, N, dz, B, N, N};
     bf16 *out = static_cast<bf16 *>(dA);
@@ -461,7 +521,6 @@ int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, 
     if (rc) return rc;
   }
   if (dB) {
-    pf::input_of_codes<<<M, 256, 0, s>>>(reinterpret_cast<const int8_t *>(a_codes), a_scale, K, a);
     if ((rc = product<2, false, false, pf::EpilogueBf16<false>>(*d, Product{K, N, M, a, dz, K, N},
                                                          {nullptr, static_cast<bf16 *>(dB), N}, s, err)))
       return rc;
@@ -483,9 +542,8 @@ int pf_dequantize_gelu_grad(int device, long long count, const unsigned char *co
   if ((rc = device_of(device, err, &d))) return rc;
   DeviceGuard g(device);
   if ((rc = stream_of(device, stream, err, &s))) return rc;
-  const unsigned grid = static_cast<unsigned>(std::min<long long>((count + 255) / 256, 1 << 20));
-  if (dst == PF_F32) pf::dequantize_grad<float><<<grid, 256, 0, s>>>(codes, count, static_cast<float *>(X));
-  else pf::dequantize_grad<bf16><<<grid, 256, 0, s>>>(codes, count, static_cast<bf16 *>(X));
+  if (dst == PF_F32) dequantize_grad<float>(codes, count, X, s);
+  else dequantize_grad<bf16>(codes, count, X, s);
   return launched(err);
 }
 

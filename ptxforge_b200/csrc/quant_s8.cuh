@@ -15,6 +15,8 @@
 #include <cuda_bf16.h>
 #include <cstdint>
 
+#include "sm100.cuh"
+
 namespace pf {
 
 constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126: scales stay normal numbers
@@ -55,78 +57,302 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
   return max(-127, min(127, q));
 }
 
-__device__ __forceinline__ float grad_value(uint32_t code) {
-  const float d = __fdiv_rn(static_cast<float>(static_cast<int>(code) - kGradZero), kGradSteps);
-  return code == kGradNan ? __uint_as_float(0x7FC00000u) : d;
+// The input's scale split into s = m 2^e, so that the backward pass rounds once where it could round twice: the
+// tensor cores take q 2^e, which is exact in bf16 (7 bits), and round(m dz), whose product is q s dz; dA, which
+// has no use for m, is divided by it at the end.  1 <= m < 2, so a token of tiny or no input keeps its dA.  A scale
+// that is not finite goes to e alone: dB is NaN then, dA is not.
+struct SplitScale {
+  float m, e;
+};
+__device__ __forceinline__ SplitScale split_scale(float s) {
+  const uint32_t b = __float_as_uint(s), field = b & 0x7F800000u;
+  if (field == 0u || field == 0x7F800000u) return {1.f, field == 0u ? s : __uint_as_float(0x7FC00000u)};
+  return {__uint_as_float((b & 0x007FFFFFu) | 0x3F800000u), __uint_as_float(b & 0xFF800000u)};
 }
 
-// Largest abs_bits of a block's threads (`sh`: one word for each warp); the result is everybody's.
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *sh) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  uint32_t m = 0;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) m = max(m, sh[w]);
-  return m;
+// The whole numbers that four codes in a word stand for: grad codes code - 26 (NaN for 255), or int8 codes.  A byte put
+// under the exponent of 2^23 is the float 2^23 + byte.
+__device__ __forceinline__ void grad_steps4(uint32_t w, float (&k)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t b = __byte_perm(w, 0x4B000000u, 0x7650 | j);
+    k[j] = b == (0x4B000000u | kGradNan) ? __uint_as_float(0x7FC00000u) : __uint_as_float(b) - (8388608.f + kGradZero);
+  }
+}
+__device__ __forceinline__ void codes4(uint32_t w, float (&q)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    q[j] = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4B000000u, 0x7650 | j)) - (8388608.f + 128.f);
+}
+// k / 200 rounded once, for every k of a code: a product by 1 / 200 and one correction by what it leaves.
+__device__ __forceinline__ float grad_value(float k) {
+  const float q = k * (1.f / kGradSteps);
+  return fmaf(fmaf(-kGradSteps, q, k), 1.f / kGradSteps, q);
 }
 
-// A scale for each row: one block a row.
-template <class T>
-__global__ void quantize_rows_s8(const T *X, long long ldx, int cols, int8_t *Q, long long ldq, float *scale) {
-  __shared__ uint32_t sh[32];
-  const long long r = blockIdx.x;
+// ------------------------------------------------------------------------------------------------
+// vectors of kVec values of a row: 16 bytes of them at once, or one
+// ------------------------------------------------------------------------------------------------
+template <int kBytes>
+struct Word;
+template <>
+struct Word<1> { typedef uint8_t type; };
+template <>
+struct Word<2> { typedef uint16_t type; };
+template <>
+struct Word<4> { typedef uint32_t type; };
+template <>
+struct Word<8> { typedef uint2 type; };
+template <>
+struct Word<16> { typedef uint4 type; };
+
+template <class T, int kVec>
+struct Values {
+  typename Word<sizeof(T) * kVec>::type w;
+  __device__ __forceinline__ void load(const T *p) { w = *reinterpret_cast<const typename Word<sizeof(T) * kVec>::type *>(p); }
+  __device__ __forceinline__ float operator[](int j) const { return to_f32(reinterpret_cast<const T *>(&w)[j]); }
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) m = max(m, abs_bits((*this)[j]));
+    return m;
+  }
+};
+
+// Codes of kVec values with the scales s[j] (all the same where kOne).  1.5 2^23 + x / s holds the code in its low byte,
+// rounded to the nearest whole number by the addition; vectors with a value near a half step are done again by
+// code_of.
+template <class T, int kVec, bool kOne>
+__device__ __forceinline__ void store_codes(const Values<T, kVec> &x, const float *s, const float *inv, int8_t *q) {
+  constexpr float magic = 12582912.f;
+  typedef Values<int8_t, kVec> Bytes;
+  union {
+    decltype(Bytes::w) w;
+    uint8_t b[kVec];
+  } u;
+  bool near = false;
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    const float t = x[j] * inv[kOne ? 0 : j];
+    const float r = t + magic;
+    near |= fabsf(t - (r - magic)) > 0.5f - 3e-5f;
+    u.b[j] = static_cast<uint8_t>(__float_as_uint(r));
+  }
+  if (near) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) u.b[j] = static_cast<uint8_t>(code_of(x[j], s[kOne ? 0 : j], inv[kOne ? 0 : j]));
+  }
+#pragma unroll
+  for (int j = 0; j < kVec; ++j)
+    if (s[kOne ? 0 : j] != s[kOne ? 0 : j]) u.b[j] = 0;
+  *reinterpret_cast<decltype(u.w) *>(q) = u.w;
+}
+
+// ------------------------------------------------------------------------------------------------
+// a scale for each row
+// ------------------------------------------------------------------------------------------------
+// blockDim.x threads a row and blockDim.y rows a block (a warp's 32 threads where there are several), kHeld vectors a
+// thread held in registers: one pass over X.  What a longer row has beyond them is read again (from L2).
+template <class T, int kVec, int kHeld>
+__global__ void __launch_bounds__(512) quantize_rows_s8(const T *X, long long ldx, int rows, int cols, int8_t *Q,
+                                                        long long ldq, float *scale) {
+  __shared__ uint32_t sh[16];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (r >= rows) return;  // whole warps: blockDim.y > 1 only with a warp a row
   const T *x = X + r * ldx;
+  const int vecs = cols / kVec, step = blockDim.x;
+  Values<T, kVec> held[kHeld];
   uint32_t m = 0;
-  for (int c = threadIdx.x; c < cols; c += blockDim.x) m = max(m, abs_bits(to_f32(x[c])));
-  const float s = scale_of(block_max(m, sh)), inv = __fdiv_rn(1.f, s);
-  for (int c = threadIdx.x; c < cols; c += blockDim.x)
-    Q[r * ldq + c] = static_cast<int8_t>(code_of(to_f32(x[c]), s, inv));
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int v = threadIdx.x + i * step;
+    if (v < vecs) held[i].load(x + static_cast<long long>(v) * kVec);
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (static_cast<int>(threadIdx.x) + i * step < vecs) m = max(m, held[i].amax());
+  for (int v = threadIdx.x + kHeld * step; v < vecs; v += step) {
+    Values<T, kVec> y;
+    y.load(x + static_cast<long long>(v) * kVec);
+    m = max(m, y.amax());
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (blockDim.x > 32) {
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = 0;
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) m = max(m, sh[w]);
+  }
+  const float s = scale_of(m), inv = __fdiv_rn(1.f, s);
+  int8_t *q = Q + r * ldq;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int v = threadIdx.x + i * step;
+    if (v < vecs) store_codes<T, kVec, true>(held[i], &s, &inv, q + static_cast<long long>(v) * kVec);
+  }
+  for (int v = threadIdx.x + kHeld * step; v < vecs; v += step) {
+    Values<T, kVec> y;
+    y.load(x + static_cast<long long>(v) * kVec);
+    store_codes<T, kVec, true>(y, &s, &inv, q + static_cast<long long>(v) * kVec);
+  }
   if (threadIdx.x == 0) scale[r] = s;
 }
 
-// A scale for each column: 32 columns a block of 32 x 8 threads.
-template <class T>
-__global__ void scale_cols_s8(const T *X, long long ldx, int rows, int cols, float *scale) {
-  __shared__ uint32_t sh[8][32];
-  const int c = blockIdx.x * 32 + threadIdx.x;
-  uint32_t m = 0;
-  if (c < cols)
-    for (long long r = threadIdx.y; r < rows; r += 8) m = max(m, abs_bits(to_f32(X[r * ldx + c])));
-  sh[threadIdx.y][threadIdx.x] = m;
+// ------------------------------------------------------------------------------------------------
+// a scale for each column
+// ------------------------------------------------------------------------------------------------
+// A cluster takes a strip of 128 bytes of columns, each of its CTAs a share of the rows, of which it holds `held` in
+// shared memory: one pass over X.  The column maxima are joined through distributed shared memory.  What a longer share
+// has beyond the held rows is read again.
+template <class T, int kVec>
+__global__ void __launch_bounds__(256) quantize_cols_s8(const T *X, long long ldx, int rows, int cols, int held, int8_t *Q,
+                                                        long long ldq, float *scale) {
+  constexpr int W = 128 / sizeof(T), LANES = W / kVec, STEP = 256 / LANES;  // columns; threads a row; rows at once
+  typedef Values<T, kVec> Vec;
+  extern __shared__ uint4 slab4[];
+  T *slab = reinterpret_cast<T *>(slab4);
+  __shared__ uint32_t amax[W];
+  uint32_t splits;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+  const int rank = static_cast<int>(cluster_ctarank());
+  const long long r0 = static_cast<long long>(rows) * rank / splits, r1 = static_cast<long long>(rows) * (rank + 1) / splits;
+  const int n = static_cast<int>(r1 - r0);
+  const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES;
+  const long long c = static_cast<long long>(blockIdx.x / splits) * W + lane * kVec;
+  const bool inside = c < cols;  // whole vectors: cols is a multiple of kVec
+  const T *x = X + r0 * ldx + c;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  if (threadIdx.x < W) amax[threadIdx.x] = 0;
   __syncthreads();
-  if (threadIdx.y == 0 && c < cols) {
-    for (int i = 1; i < 8; ++i) m = max(m, sh[i][threadIdx.x]);
-    scale[c] = scale_of(m);
+  uint32_t m[kVec] = {};
+  if (inside) {
+#pragma unroll 8
+    for (int r = first; r < n; r += STEP) {
+      Vec y;
+      y.load(x + r * ldx);
+      if (r < held) *reinterpret_cast<decltype(y.w) *>(slab + r * W + lane * kVec) = y.w;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) m[j] = max(m[j], abs_bits(y[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) atomicMax(&amax[lane * kVec + j], m[j]);
   }
-}
-template <class T>
-__global__ void quantize_cols_s8(const T *X, long long ldx, int cols, const float *scale, int8_t *Q, long long ldq) {
-  const long long r = blockIdx.x;
-  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-    const float s = scale[c];
-    Q[r * ldq + c] = static_cast<int8_t>(code_of(to_f32(X[r * ldx + c]), s, __fdiv_rn(1.f, s)));
+  __syncwarp();
+  cluster_sync();
+  if (inside) {
+    float s[kVec], inv[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      uint32_t all = 0;
+      for (uint32_t k = 0; k < splits; ++k) all = max(all, ld_cluster(mapa_shared(smem_u32(&amax[lane * kVec + j]), k)));
+      s[j] = scale_of(all);
+      inv[j] = __fdiv_rn(1.f, s[j]);
+      if (rank == 0 && first == 0) scale[c + j] = s[j];
+    }
+    int8_t *q = Q + r0 * ldq + c;
+#pragma unroll 4
+    for (int r = first; r < n; r += STEP) {
+      Vec y;
+      if (r < held) y.w = *reinterpret_cast<const decltype(y.w) *>(slab + r * W + lane * kVec);
+      else y.load(x + r * ldx);
+      store_codes<T, kVec, false>(y, s, inv, q + r * ldq);
+    }
   }
+  __syncwarp();
+  cluster_sync();  // nobody leaves while its maxima may be read
 }
 
+// ------------------------------------------------------------------------------------------------
+// back from codes
+// ------------------------------------------------------------------------------------------------
 template <class T>
-__global__ void dequantize_s8(const int8_t *Q, long long ldq, int cols, const float *scale, int by_row, T *X,
-                              long long ldx) {
-  const long long r = blockIdx.x;
-  for (int c = threadIdx.x; c < cols; c += blockDim.x)
-    X[r * ldx + c] = from_f32<T>(static_cast<float>(Q[r * ldq + c]) * scale[by_row ? r : c]);
+__device__ __forceinline__ void store8(T *out, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4 *>(out) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                                 pack_bf16x2(x[6], x[7]));
+  } else {
+    reinterpret_cast<float4 *>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4 *>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+__device__ __forceinline__ void codes8(uint2 w, float (&q)[8]) {
+  float a[4], b[4];
+  codes4(w.x, a);
+  codes4(w.y, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) q[j] = a[j], q[j + 4] = b[j];
 }
 
-template <class T>
-__global__ void dequantize_grad(const uint8_t *D, long long n, T *X) {
-  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n;
-       i += static_cast<long long>(gridDim.x) * blockDim.x)
-    X[i] = from_f32<T>(grad_value(D[i]));
+// Scale of a row or of the columns; kInput: the part 2^e of a row's (split_scale), which keeps the values exact in bf16.
+// kVec 8 or 1.  blockDim.x threads a row, blockDim.y rows a block.
+template <class T, int kVec, bool kByRow, bool kInput = false>
+__device__ __forceinline__ void restore_row(const int8_t *q, int cols, const float *scale, T *x, int first, int step) {
+  float s = kByRow ? __ldg(scale) : 0.f;
+  if constexpr (kInput) s = split_scale(s).e;
+  if constexpr (kVec == 8) {
+#pragma unroll 4
+    for (int c = first * 8; c < cols; c += step * 8) {
+      float v[8];
+      codes8(*reinterpret_cast<const uint2 *>(q + c), v);
+      if constexpr (kByRow) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= s;
+      } else if ((reinterpret_cast<uintptr_t>(scale) & 15) == 0) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(scale + c)), b = __ldg(reinterpret_cast<const float4 *>(scale + c) + 1);
+        v[0] *= a.x, v[1] *= a.y, v[2] *= a.z, v[3] *= a.w;
+        v[4] *= b.x, v[5] *= b.y, v[6] *= b.z, v[7] *= b.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= __ldg(scale + c + j);
+      }
+      store8(x + c, v);
+    }
+  } else {
+    for (int c = first; c < cols; c += step) x[c] = from_f32<T>(static_cast<float>(q[c]) * (kByRow ? s : __ldg(scale + c)));
+  }
+}
+template <class T, int kVec, bool kByRow>
+__global__ void __launch_bounds__(256) dequantize_s8(const int8_t *Q, long long ldq, int rows, int cols, const float *scale,
+                                                     T *X, long long ldx) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (r < rows) restore_row<T, kVec, kByRow>(Q + r * ldq, cols, kByRow ? scale + r : scale, X + r * ldx, threadIdx.x, blockDim.x);
+}
+
+template <class T, int kVec>
+__global__ void __launch_bounds__(256) dequantize_grad(const uint8_t *D, long long n, T *X) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const long long stride = static_cast<long long>(gridDim.x) * 256 * kVec;
+  for (long long i = (blockIdx.x * 256ll + threadIdx.x) * kVec; i < n; i += stride) {
+    if (kVec == 8 && i + 8 <= n) {
+      const uint2 w = *reinterpret_cast<const uint2 *>(D + i);
+      float a[4], b[4], v[8];
+      grad_steps4(w.x, a);
+      grad_steps4(w.y, b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = grad_value(a[j]), v[j + 4] = grad_value(b[j]);
+      store8(X + i, v);
+    } else {
+      for (long long j = i; j < n && j < i + kVec; ++j) {
+        float k[4];
+        grad_steps4(D[j], k);
+        X[j] = from_f32<T>(grad_value(k[0]));
+      }
+    }
+  }
 }
 
 // Rows of bytes that start anywhere -> rows of whole 16-byte words.  Each word is put together from the aligned
 // 4-byte words that hold its bytes; a word with no byte of the row is not read.  What follows a row's end is whatever
 // shares its last word, and is never used.
 __global__ void align_rows(const uint8_t *X, long long ld, int cols, uint4 *Y, long long ld_y) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   const long long r = blockIdx.x;
   const uintptr_t row = reinterpret_cast<uintptr_t>(X + r * ld);
   const unsigned shift = 8 * static_cast<unsigned>(row & 3);
@@ -141,49 +367,82 @@ __global__ void align_rows(const uint8_t *X, long long ld, int cols, uint4 *Y, l
   }
 }
 
-// The input's scale split into s = m 2^e, so that the backward pass rounds once where it could round twice: the
-// tensor cores take q 2^e, which is exact in bf16 (7 bits), and round(m dz), whose product is q s dz; dA, which
-// has no use for m, is divided by it at the end.  1 <= m < 2, so a token of tiny or no input keeps its dA.  A scale
-// that is not finite goes to e alone: dB is NaN then, dA is not.
-struct SplitScale {
-  float m, e;
-};
-__device__ __forceinline__ SplitScale split_scale(float s) {
-  const uint32_t b = __float_as_uint(s), field = b & 0x7F800000u;
-  if (field == 0u || field == 0x7F800000u) return {1.f, field == 0u ? s : __uint_as_float(0x7FC00000u)};
-  return {__uint_as_float((b & 0x007FFFFFu) | 0x3F800000u), __uint_as_float(b & 0xFF800000u)};
+// ------------------------------------------------------------------------------------------------
+// the backward pass's elementwise part
+// ------------------------------------------------------------------------------------------------
+// Blocks below dz_blocks: m dz = m dC d~ (rounded once to bf16) of 256 columns x kDzRows rows and, from the unrounded dz,
+// their column sums in fp32 (`sums` [row block][column]; with one row block that is dbias).  dC k is exact in fp32 (8 by
+// 8 bits), so dz is rounded once by 1 / 200.  The blocks after them: the input's q 2^e in bf16, exact, a row each.
+// a_scale may be null (m = 1, no input wanted).
+constexpr int kDzRows = 128, kDzCols = 256;
+__global__ void __launch_bounds__(256) backward_operands(const __nv_bfloat16 *dC, const uint8_t *D, const float *a_scale,
+                                                         int M, int N, int dz_blocks, int col_blocks, __nv_bfloat16 *dz,
+                                                         float *sums, const int8_t *Q, int K, __nv_bfloat16 *input) {
+  __shared__ float sh[8][kDzCols];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  if (static_cast<int>(blockIdx.x) >= dz_blocks) {
+    const long long r = blockIdx.x - dz_blocks;
+    restore_row<__nv_bfloat16, 8, true, true>(Q + r * K, K, a_scale + r, input + r * K, threadIdx.x, 256);
+    return;
+  }
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int rb = blockIdx.x / col_blocks;
+  const int c = (blockIdx.x - rb * col_blocks) * kDzCols + lane * 8;
+  float sum[8] = {};
+  if (c < N) {
+    const int r0 = rb * kDzRows + row, r1 = min(M, (rb + 1) * kDzRows);
+#pragma unroll 4
+    for (int r = r0; r < r1; r += 8) {
+      const long long i = static_cast<long long>(r) * N + c;
+      const uint4 g = *reinterpret_cast<const uint4 *>(dC + i);
+      const uint2 w = *reinterpret_cast<const uint2 *>(D + i);
+      const float m = a_scale ? split_scale(__ldg(a_scale + r)).m : 1.f;
+      float a[4], b[4], v[8];
+      grad_steps4(w.x, a);
+      grad_steps4(w.y, b);
+      const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = __uint_as_float((j & 1) ? gw[j / 2] & 0xFFFF0000u : gw[j / 2] << 16);
+        const float z = x * (j < 4 ? a[j & 3] : b[j & 3]) * (1.f / kGradSteps);
+        sum[j] += z;
+        v[j] = z * m;
+      }
+      store8(dz + i, v);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sh[row][lane * 8 + j] = sum[j];
+  __syncthreads();
+  const int col = (blockIdx.x - rb * col_blocks) * kDzCols + threadIdx.x;
+  if (col < N) {
+    float total = sh[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) total += sh[i][threadIdx.x];
+    sums[static_cast<long long>(rb) * N + col] = total;
+  }
 }
 
-// m dz = m dC d~ (rounded once to bf16) and, from the unrounded dz, the column sums of `kDzRows` rows in fp32:
-// partial[blockIdx.y][column].  a_scale may be null: m = 1.
-constexpr int kDzRows = 128;
-__global__ void gelu_backward_dz(const __nv_bfloat16 *dC, const uint8_t *D, const float *a_scale, int M, int N,
-                                 __nv_bfloat16 *dz, float *partial) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= N) return;
-  const int r1 = min(M, static_cast<int>(blockIdx.y + 1) * kDzRows);
+// dbias: the row blocks' sums added, eight runs of them side by side, then the runs in order.
+__global__ void __launch_bounds__(256) sum_row_blocks(const float *sums, int blocks, int N, float *out) {
+  __shared__ float sh[8][32];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
   float sum = 0.f;
-  for (int r = blockIdx.y * kDzRows; r < r1; ++r) {
-    const long long i = static_cast<long long>(r) * N + c;
-    const float v = to_f32(dC[i]) * grad_value(D[i]);
-    dz[i] = __float2bfloat16_rn(a_scale ? v * split_scale(a_scale[r]).m : v);
-    sum += v;
+  if (c < N) {
+#pragma unroll 8
+    for (int b = run; b < blocks; b += 8) sum += sums[static_cast<long long>(b) * N + c];
   }
-  partial[static_cast<long long>(blockIdx.y) * N + c] = sum;
-}
-// q 2^e in bf16, exact.
-__global__ void input_of_codes(const int8_t *Q, const float *a_scale, int K, __nv_bfloat16 *X) {
-  const long long r = blockIdx.x;
-  const float e = split_scale(a_scale[r]).e;
-  for (int c = threadIdx.x; c < K; c += blockDim.x) X[r * K + c] = __float2bfloat16_rn(static_cast<float>(Q[r * K + c]) * e);
-}
-// dbias: the partial column sums added in row order.
-__global__ void sum_partials(const float *partial, int parts, int N, float *out) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= N) return;
-  float sum = 0.f;
-  for (int p = 0; p < parts; ++p) sum += partial[static_cast<long long>(p) * N + c];
-  out[c] = sum;
+  sh[run][lane] = sum;
+  __syncthreads();
+  if (run == 0 && c < N) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum += sh[i][lane];
+    out[c] = sum;
+  }
 }
 
 }  // namespace pf
