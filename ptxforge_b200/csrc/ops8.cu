@@ -60,14 +60,15 @@ struct Err {
 
 // The device's properties, looked up once; a failed look-up is tried again by the next call.
 int device_of(int device, const Err &err, Device **out) {
-  int n = 0;
-  if (cudaGetDeviceCount(&n) != cudaSuccess || device < 0 || device >= n || device >= kMaxDevices) {
-    cudaGetLastError();
-    return err(PF_ENODEV, "no CUDA device %d", device);
-  }
+  if (device < 0 || device >= kMaxDevices) return err(PF_ENODEV, "no CUDA device %d", device);
   Device &d = g_devices[device];
   std::lock_guard<std::mutex> lk(d.mu);
   if (!d.ready) {
+    int n = 0;
+    if (cudaGetDeviceCount(&n) != cudaSuccess || device >= n) {
+      cudaGetLastError();
+      return err(PF_ENODEV, "no CUDA device %d", device);
+    }
     DeviceGuard g(device);
     void *p = nullptr;
     cudaError_t e = cudaDeviceGetAttribute(&d.cc_major, cudaDevAttrComputeCapabilityMajor, device);

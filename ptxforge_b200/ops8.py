@@ -20,21 +20,29 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import threading
 from typing import NamedTuple
 
 import ptxforge_b200 as _pf
 
 _F32, _BF16 = 0, 2  # pf_dtype
 _ERR_BYTES = 256
+_local = threading.local()  # each thread's error text
+_here = contextlib.nullcontext()
+torch = None  # imported by the first call: the package loads without it
+_raw_stream = None  # torch's current stream of a device index, as a handle
 
 
-def _torch():
-    import torch
-    return torch
+def _need_torch():
+    global torch, _raw_stream
+    if torch is None:
+        import torch as t
+        # the handle without a Stream object around it, where torch has that: 2 us less a call
+        _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (lambda i: t.cuda.current_stream(i).cuda_stream)
+        torch = t
 
 
 def _type_code(dtype, what: str) -> int:
-    torch = _torch()
     if dtype is torch.bfloat16:
         return _BF16
     if dtype is torch.float32:
@@ -44,44 +52,43 @@ def _type_code(dtype, what: str) -> int:
 
 def _matrix(x, name: str, dtype=None, shape=None, device=None, contiguous: bool = False):
     """(rows, cols, row stride) of a CUDA matrix with contiguous rows, or ValueError."""
-    if x.dim() != 2:
-        raise ValueError(f"{name} must be a matrix, got {tuple(x.shape)}")
+    size = x.shape
+    if len(size) != 2:
+        raise ValueError(f"{name} must be a matrix, got {tuple(size)}")
     _check(x, name, dtype, shape, device)
-    rows, cols = x.shape
-    if rows == 0 or cols == 0:
+    rows, cols = size
+    if x.is_contiguous():
         return rows, cols, cols
     ld, step = x.stride()
-    if rows == 1:
-        ld = cols
-    if (step != 1 and cols > 1) or ld < cols or (contiguous and ld != cols):
+    if contiguous or (step != 1 and cols > 1) or ld < cols:
         raise ValueError(f"{name} must be contiguous" + ("" if contiguous else " along its rows, which must not overlap")
                          + f", got strides {x.stride()}")
     return rows, cols, ld
 
 
 def _vector(x, name: str, n: int, device):
-    torch = _torch()
     _check(x, name, torch.float32, (n,), device)
     if not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
 def _check(x, name, dtype, shape, device):
+    """`device`: the index of the other operands' device, None for the first."""
     if dtype is not None and x.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {x.dtype}")
-    if shape is not None and tuple(x.shape) != tuple(shape):
+    if shape is not None and x.shape != shape:
         raise ValueError(f"{name} must be {' x '.join(map(str, shape))}, got {tuple(x.shape)}")
-    if not x.is_cuda:
+    at = x.get_device()
+    if at < 0:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if device is not None and x.device != device:
-        raise ValueError(f"{name} is on {x.device}, other operands on {device}")
+    if device is not None and at != device:
+        raise ValueError(f"{name} is on cuda:{at}, other operands on cuda:{device}")
 
 
 def _on(stream, device):
     """(the stream's handle, a context in which torch allocates on that stream)."""
-    torch = _torch()
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, contextlib.nullcontext()
+        return _raw_stream(device), _here
     handle = _pf._stream(stream)
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
@@ -89,7 +96,9 @@ def _on(stream, device):
 
 
 def _call(name: str, *args):
-    err = ctypes.create_string_buffer(_ERR_BYTES)
+    err = getattr(_local, "err", None)
+    if err is None:
+        err = _local.err = ctypes.create_string_buffer(_ERR_BYTES)
     rc = getattr(_pf.load_library(), name)(*args, err, _ERR_BYTES)
     if rc:
         raise _pf.PFError(rc, f"{name}: {err.value.decode()}")
@@ -106,36 +115,38 @@ def quantize_s8(X, axis: int = 1, codes=None, scale=None, *, stream=None):
     max(max |x| / 127, 2**-126), one for each row (axis 1, a token) or column (axis 0, a channel).
 
     A row (column) with an infinity or NaN gets the scale NaN and codes 0.  Row strides are free."""
-    torch = _torch()
+    _need_torch()
     src = _type_code(X.dtype, "X")
     rows, cols, ldx = _matrix(X, "X")
     n = _axis(axis, rows, cols)
-    handle, here = _on(stream, X.device)
+    dev = X.get_device()
+    handle, here = _on(stream, dev)
     with here:
         if codes is None:
             codes = torch.empty((rows, cols), dtype=torch.int8, device=X.device)
         if scale is None:
             scale = torch.empty(n, dtype=torch.float32, device=X.device)
-    ldq = _matrix(codes, "codes", torch.int8, (rows, cols), X.device)[2]
-    _vector(scale, "scale", n, X.device)
-    _call("pf_quantize_s8", X.device.index, src, rows, cols, X.data_ptr(), ldx, axis, codes.data_ptr(), ldq,
+    ldq = _matrix(codes, "codes", torch.int8, (rows, cols), dev)[2]
+    _vector(scale, "scale", n, dev)
+    _call("pf_quantize_s8", dev, src, rows, cols, X.data_ptr(), ldx, axis, codes.data_ptr(), ldq,
           scale.data_ptr(), handle)
     return codes, scale
 
 
 def dequantize_s8(codes, scale, axis: int = 1, out=None, *, dtype=None, stream=None):
     """The values codes * scale stand for, in `dtype` (that of `out`, else bfloat16).  Row strides are free."""
-    torch = _torch()
+    _need_torch()
     rows, cols, ldq = _matrix(codes, "codes", torch.int8)
-    _vector(scale, "scale", _axis(axis, rows, cols), codes.device)
+    dev = codes.get_device()
+    _vector(scale, "scale", _axis(axis, rows, cols), dev)
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
     dst = _type_code(dtype, "dtype")
-    handle, here = _on(stream, codes.device)
+    handle, here = _on(stream, dev)
     if out is None:
         with here:
             out = torch.empty((rows, cols), dtype=dtype, device=codes.device)
-    ldx = _matrix(out, "out", dtype, (rows, cols), codes.device)[2]
-    _call("pf_dequantize_s8", codes.device.index, rows, cols, codes.data_ptr(), ldq, scale.data_ptr(), axis, dst,
+    ldx = _matrix(out, "out", dtype, (rows, cols), dev)[2]
+    _call("pf_dequantize_s8", dev, rows, cols, codes.data_ptr(), ldq, scale.data_ptr(), axis, dst,
           out.data_ptr(), ldx, handle)
     return out
 
@@ -145,28 +156,29 @@ def gemm_s8(A, B, scale_a, scale_b, bias=None, C=None, *, gelu: bool = False, dt
     scale for each token), scale_b float32 [N] (for each channel), bias float32 [N] or None; f is GELU's tanh form with
     gelu=True, else the identity.  `dtype` of C: bfloat16 (default) or float32.  The integer sums are exact; K is at
     most 131071.  Any M, N, K; row strides are free."""
-    torch = _torch()
+    _need_torch()
     M, K, lda = _matrix(A, "A", torch.int8)
-    K2, N, ldb = _matrix(B, "B", torch.int8, None, A.device)
+    dev = A.get_device()
+    K2, N, ldb = _matrix(B, "B", torch.int8, None, dev)
     if K2 != K:
         raise ValueError(f"shape mismatch: A {tuple(A.shape)}, B {tuple(B.shape)}")
-    _vector(scale_a, "scale_a", M, A.device)
-    _vector(scale_b, "scale_b", N, A.device)
+    _vector(scale_a, "scale_a", M, dev)
+    _vector(scale_b, "scale_b", N, dev)
     if bias is not None:
-        _vector(bias, "bias", N, A.device)
+        _vector(bias, "bias", N, dev)
     dtype = dtype or (C.dtype if C is not None else torch.bfloat16)
     out = _type_code(dtype, "dtype")
-    handle, here = _on(stream, A.device)
+    handle, here = _on(stream, dev)
     if C is None:
         with here:
             C = torch.empty((M, N), dtype=dtype, device=A.device)
-    ldc = _matrix(C, "C", dtype, (M, N), A.device)[2]
+    ldc = _matrix(C, "C", dtype, (M, N), dev)[2]
     a, b, space = A.data_ptr(), B.data_ptr(), None
     size = _pf.load_library().pf_gemm_s8_workspace(M, N, K, a, lda, b, ldb)  # 0 where rows start on 16-byte boundaries
     if size:
         with here:
             space = torch.empty(size, dtype=torch.uint8, device=A.device)  # back to the stream's pool on return
-    _call("pf_gemm_s8", A.device.index, M, N, K, a, lda, b, ldb, scale_a.data_ptr(), scale_b.data_ptr(),
+    _call("pf_gemm_s8", dev, M, N, K, a, lda, b, ldb, scale_a.data_ptr(), scale_b.data_ptr(),
           None if bias is None else bias.data_ptr(), int(gelu), out, C.data_ptr(), ldc,
           None if space is None else space.data_ptr(), size, handle)
     return C
@@ -192,21 +204,22 @@ def gemm_bias_gelu_checkpoint(A, B, bias, C=None, *, keep_input: bool = True, st
     """(C, checkpoint): C = gelu_tanh(A @ B + bias) in bfloat16, for bfloat16 A [M, K] and B [K, N] and float32 bias [N],
     and in 8 bits what gemm_bias_gelu_backward needs.  keep_input=False leaves the input out (no dB then).  Operands
     contiguous, N and K multiples of 8."""
-    torch = _torch()
+    _need_torch()
     M, K, _ = _matrix(A, "A", torch.bfloat16, contiguous=True)
-    K2, N, _ = _matrix(B, "B", torch.bfloat16, None, A.device, contiguous=True)
+    dev = A.get_device()
+    K2, N, _ = _matrix(B, "B", torch.bfloat16, None, dev, contiguous=True)
     if K2 != K:
         raise ValueError(f"shape mismatch: A {tuple(A.shape)}, B {tuple(B.shape)}")
-    _vector(bias, "bias", N, A.device)
-    handle, here = _on(stream, A.device)
+    _vector(bias, "bias", N, dev)
+    handle, here = _on(stream, dev)
     with here:
         if C is None:
             C = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
         grad_codes = torch.empty((M, N), dtype=torch.uint8, device=A.device)
         a_codes = torch.empty((M, K), dtype=torch.int8, device=A.device) if keep_input else None
         a_scale = torch.empty(M, dtype=torch.float32, device=A.device) if keep_input else None
-    _matrix(C, "C", torch.bfloat16, (M, N), A.device, contiguous=True)
-    _call("pf_gemm_bias_gelu_checkpoint", A.device.index, M, N, K, A.data_ptr(), B.data_ptr(), bias.data_ptr(), C.data_ptr(),
+    _matrix(C, "C", torch.bfloat16, (M, N), dev, contiguous=True)
+    _call("pf_gemm_bias_gelu_checkpoint", dev, M, N, K, A.data_ptr(), B.data_ptr(), bias.data_ptr(), C.data_ptr(),
           a_codes.data_ptr() if keep_input else None, a_scale.data_ptr() if keep_input else None, grad_codes.data_ptr(),
           handle)
     return C, Checkpoint(a_codes, a_scale, grad_codes)
@@ -216,28 +229,29 @@ def gemm_bias_gelu_backward(dC, B, checkpoint: Checkpoint, *, need=("dA", "dB", 
     """(dA, dB, dbias) of C = gelu_tanh(A @ B + bias) from dC [M, N] (bfloat16), B and the forward pass's checkpoint:
     bfloat16 [M, K] and [K, N], float32 [N]; None for those that `need` leaves out.  Sums are in float32, in an order
     that depends on the sizes alone."""
-    torch = _torch()
+    _need_torch()
     unknown = set(need) - {"dA", "dB", "dbias"}
     if unknown:
         raise ValueError(f"need names dA, dB and dbias, got {sorted(unknown)}")
     M, N, _ = _matrix(dC, "dC", torch.bfloat16, contiguous=True)
-    K, _, _ = _matrix(B, "B", torch.bfloat16, (B.shape[0], N), dC.device, contiguous=True)
-    _matrix(checkpoint.grad_codes, "checkpoint.grad_codes", torch.uint8, (M, N), dC.device, contiguous=True)
+    dev = dC.get_device()
+    K, _, _ = _matrix(B, "B", torch.bfloat16, (B.shape[0], N), dev, contiguous=True)
+    _matrix(checkpoint.grad_codes, "checkpoint.grad_codes", torch.uint8, (M, N), dev, contiguous=True)
     a, s = None, None
     if "dB" in need:
         if checkpoint.a_codes is None:
             raise ValueError("dB needs the input: the checkpoint was made with keep_input=False")
-        _matrix(checkpoint.a_codes, "checkpoint.a_codes", torch.int8, (M, K), dC.device, contiguous=True)
-        _vector(checkpoint.a_scale, "checkpoint.a_scale", M, dC.device)
+        _matrix(checkpoint.a_codes, "checkpoint.a_codes", torch.int8, (M, K), dev, contiguous=True)
+        _vector(checkpoint.a_scale, "checkpoint.a_scale", M, dev)
         a, s = checkpoint.a_codes.data_ptr(), checkpoint.a_scale.data_ptr()
-    handle, here = _on(stream, dC.device)
+    handle, here = _on(stream, dev)
     size = _pf.load_library().pf_gemm_bias_gelu_backward_workspace(M, N, K)
     with here:
         dA = torch.empty((M, K), dtype=torch.bfloat16, device=dC.device) if "dA" in need else None
         dB = torch.empty((K, N), dtype=torch.bfloat16, device=dC.device) if "dB" in need else None
         dbias = torch.empty(N, dtype=torch.float32, device=dC.device) if "dbias" in need else None
         space = torch.empty(size, dtype=torch.uint8, device=dC.device)  # back to the stream's pool on return
-    _call("pf_gemm_bias_gelu_backward", dC.device.index, M, N, K, dC.data_ptr(), B.data_ptr(), a, s,
+    _call("pf_gemm_bias_gelu_backward", dev, M, N, K, dC.data_ptr(), B.data_ptr(), a, s,
           checkpoint.grad_codes.data_ptr(), None if dA is None else dA.data_ptr(), None if dB is None else dB.data_ptr(),
           None if dbias is None else dbias.data_ptr(), space.data_ptr(), size, handle)
     return dA, dB, dbias
@@ -245,20 +259,21 @@ def gemm_bias_gelu_backward(dC, B, checkpoint: Checkpoint, *, need=("dA", "dB", 
 
 def dequantize_gelu_grad(codes, out=None, *, dtype=None, stream=None):
     """The GELU derivatives (code - 26) / 200 that uint8 codes stand for (NaN for 255), in `dtype` (default bfloat16)."""
-    torch = _torch()
+    _need_torch()
     _check(codes, "codes", torch.uint8, None, None)
     if not codes.is_contiguous():
         raise ValueError("codes must be contiguous")
+    dev = codes.get_device()
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
     dst = _type_code(dtype, "dtype")
-    handle, here = _on(stream, codes.device)
+    handle, here = _on(stream, dev)
     if out is None:
         with here:
             out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-    _check(out, "out", dtype, codes.shape, codes.device)
+    _check(out, "out", dtype, codes.shape, dev)
     if not out.is_contiguous():
         raise ValueError("out must be contiguous")
-    _call("pf_dequantize_gelu_grad", codes.device.index, codes.numel(), codes.data_ptr(), dst, out.data_ptr(), handle)
+    _call("pf_dequantize_gelu_grad", dev, codes.numel(), codes.data_ptr(), dst, out.data_ptr(), handle)
     return out
 
 
