@@ -212,17 +212,20 @@ template <class T>
 void dequantize(const int8_t *q, long long ldq, int rows, int cols, const float *scale, int axis, void *X, long long ldx,
                 cudaStream_t s) {
   T *x = static_cast<T *>(X);
-  if (vectors_fit(q, ldq, cols, 1, 8) && vectors_fit(X, ldx, cols, sizeof(T), 8)) dequantize<T, 8>(q, ldq, rows, cols, scale, axis, x, ldx, s);
+  constexpr int kVec = 16 / sizeof(T);
+  if (vectors_fit(q, ldq, cols, 1, kVec) && vectors_fit(X, ldx, cols, sizeof(T), kVec))
+    dequantize<T, kVec>(q, ldq, rows, cols, scale, axis, x, ldx, s);
   else dequantize<T, 1>(q, ldq, rows, cols, scale, axis, x, ldx, s);
 }
 
 template <class T>
 void dequantize_grad(const unsigned char *codes, long long n, void *X, cudaStream_t s) {
   T *x = static_cast<T *>(X);
-  const bool wide = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && pf::aligned16(X);
-  const int per = 256 * (wide ? 8 : 1);
+  constexpr int kVec = 16 / sizeof(T);
+  const bool wide = reinterpret_cast<uintptr_t>(codes) % kVec == 0 && pf::aligned16(X);
+  const int per = 256 * (wide ? kVec : 1);
   const dim3 grid(static_cast<unsigned>(std::min<long long>((n + per - 1) / per, 1 << 30)));
-  pf::launch_pdl(wide ? &pf::dequantize_grad<T, 8> : &pf::dequantize_grad<T, 1>, grid, 256, 0, s, codes, n, x);
+  pf::launch_pdl(wide ? &pf::dequantize_grad<T, kVec> : &pf::dequantize_grad<T, 1>, grid, 256, 0, s, codes, n, x);
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }

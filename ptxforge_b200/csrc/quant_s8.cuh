@@ -111,41 +111,77 @@ struct Values {
   typename Word<sizeof(T) * kVec>::type w;
   __device__ __forceinline__ void load(const T *p) { w = *reinterpret_cast<const typename Word<sizeof(T) * kVec>::type *>(p); }
   __device__ __forceinline__ float operator[](int j) const { return to_f32(reinterpret_cast<const T *>(&w)[j]); }
-  __device__ __forceinline__ uint32_t amax() const {
-    uint32_t m = 0;
+};
+
+// Largest |x| of vectors, NaN where there is one; eight bf16 values go two to an instruction.
+template <class T, int kVec>
+struct Largest {
+  uint32_t m = 0;
+  __device__ __forceinline__ void take(const Values<T, kVec> &x) {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) m = max(m, abs_bits((*this)[j]));
-    return m;
+    for (int j = 0; j < kVec; ++j) m = max(m, abs_bits(x[j]));
+  }
+  __device__ __forceinline__ uint32_t bits() const { return m; }
+};
+template <>
+struct Largest<__nv_bfloat16, 8> {
+  __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
+  __device__ __forceinline__ void take(const Values<__nv_bfloat16, 8> &x) {
+    const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&x.w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = __hmax2_nan(m, __habs2(p[j]));
+  }
+  __device__ __forceinline__ uint32_t bits() const {
+    return max(abs_bits(__low2float(m)), abs_bits(__high2float(m)));
   }
 };
 
-// Codes of kVec values with the scales s[j] (all the same where kOne).  1.5 2^23 + x / s holds the code in its low byte,
+// Codes of kVec values with the scales s[j] (one for all where kOne).  1.5 2^23 + x / s holds the code in its low byte,
 // rounded to the nearest whole number by the addition; vectors with a value near a half step are done again by
-// code_of.
+// code_of.  A scale that is NaN gives code 0.
 template <class T, int kVec, bool kOne>
 __device__ __forceinline__ void store_codes(const Values<T, kVec> &x, const float *s, const float *inv, int8_t *q) {
   constexpr float magic = 12582912.f;
-  typedef Values<int8_t, kVec> Bytes;
-  union {
-    decltype(Bytes::w) w;
-    uint8_t b[kVec];
-  } u;
-  bool near = false;
+  uint32_t r[kVec];
+  float far = 0.f;
+  if constexpr (kVec == 1) {
+    const float t = x[0] * inv[0], y = t + magic;
+    far = fabsf(t - (y - magic));
+    r[0] = __float_as_uint(y);
+  } else {
 #pragma unroll
-  for (int j = 0; j < kVec; ++j) {
-    const float t = x[j] * inv[kOne ? 0 : j];
-    const float r = t + magic;
-    near |= fabsf(t - (r - magic)) > 0.5f - 3e-5f;
-    u.b[j] = static_cast<uint8_t>(__float_as_uint(r));
+    for (int j = 0; j < kVec; j += 2) {
+      const float2 i2 = kOne ? make_float2(inv[0], inv[0]) : make_float2(inv[j], inv[j + 1]);
+      const float2 t = __fmul2_rn(make_float2(x[j], x[j + 1]), i2);
+      const float2 y = __fadd2_rn(t, make_float2(magic, magic));
+      const float2 n = __fadd2_rn(make_float2(magic, magic), make_float2(-y.x, -y.y));  // minus the whole number
+      const float2 d = __fadd2_rn(t, n);
+      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+      r[j] = __float_as_uint(y.x);
+      r[j + 1] = __float_as_uint(y.y);
+    }
   }
-  if (near) {
+  bool again = far > 0.5f - 3e-5f;
+  if constexpr (kOne) {
+    again |= s[0] != s[0];
+  } else {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) u.b[j] = static_cast<uint8_t>(code_of(x[j], s[kOne ? 0 : j], inv[kOne ? 0 : j]));
+    for (int j = 0; j < kVec; ++j) again |= s[j] != s[j];
   }
+  if (again) {
 #pragma unroll
-  for (int j = 0; j < kVec; ++j)
-    if (s[kOne ? 0 : j] != s[kOne ? 0 : j]) u.b[j] = 0;
-  *reinterpret_cast<decltype(u.w) *>(q) = u.w;
+    for (int j = 0; j < kVec; ++j) r[j] = static_cast<uint32_t>(code_of(x[j], s[kOne ? 0 : j], inv[kOne ? 0 : j]));
+  }
+  if constexpr (kVec == 1) {
+    *q = static_cast<int8_t>(r[0]);
+  } else {
+    uint32_t w[kVec / 4];
+#pragma unroll
+    for (int j = 0; j < kVec; j += 4)
+      w[j / 4] = __byte_perm(__byte_perm(r[j], r[j + 1], 0x0040), __byte_perm(r[j + 2], r[j + 3], 0x0040), 0x5410);
+    if constexpr (kVec == 4) *reinterpret_cast<uint32_t *>(q) = w[0];
+    else *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[1]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -164,7 +200,7 @@ __global__ void __launch_bounds__(512) quantize_rows_s8(const T *X, long long ld
   const T *x = X + r * ldx;
   const int vecs = cols / kVec, step = blockDim.x;
   Values<T, kVec> held[kHeld];
-  uint32_t m = 0;
+  Largest<T, kVec> largest;
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     const int v = threadIdx.x + i * step;
@@ -172,13 +208,13 @@ __global__ void __launch_bounds__(512) quantize_rows_s8(const T *X, long long ld
   }
 #pragma unroll
   for (int i = 0; i < kHeld; ++i)
-    if (static_cast<int>(threadIdx.x) + i * step < vecs) m = max(m, held[i].amax());
+    if (static_cast<int>(threadIdx.x) + i * step < vecs) largest.take(held[i]);
   for (int v = threadIdx.x + kHeld * step; v < vecs; v += step) {
     Values<T, kVec> y;
     y.load(x + static_cast<long long>(v) * kVec);
-    m = max(m, y.amax());
+    largest.take(y);
   }
-  m = __reduce_max_sync(0xffffffffu, m);
+  uint32_t m = __reduce_max_sync(0xffffffffu, largest.bits());
   if (blockDim.x > 32) {
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
     __syncthreads();
@@ -268,47 +304,52 @@ __global__ void __launch_bounds__(256) quantize_cols_s8(const T *X, long long ld
 // ------------------------------------------------------------------------------------------------
 // back from codes
 // ------------------------------------------------------------------------------------------------
-template <class T>
-__device__ __forceinline__ void store8(T *out, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<uint4 *>(out) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                                                 pack_bf16x2(x[6], x[7]));
-  } else {
-    reinterpret_cast<float4 *>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4 *>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  }
+__device__ __forceinline__ void store_vec(__nv_bfloat16 *out, const float (&x)[8]) {
+  *reinterpret_cast<uint4 *>(out) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                               pack_bf16x2(x[6], x[7]));
 }
-__device__ __forceinline__ void codes8(uint2 w, float (&q)[8]) {
-  float a[4], b[4];
-  codes4(w.x, a);
-  codes4(w.y, b);
+__device__ __forceinline__ void store_vec(float *out, const float (&x)[4]) {
+  *reinterpret_cast<float4 *>(out) = make_float4(x[0], x[1], x[2], x[3]);
+}
+// What the codes of one vector stand for, by codes4 or grad_steps4.
+template <int kVec, class Four>
+__device__ __forceinline__ void load_codes(const void *p, float (&q)[kVec], Four four) {
+  typename Word<kVec>::type w = *reinterpret_cast<const typename Word<kVec>::type *>(p);
+  const uint32_t *words = reinterpret_cast<const uint32_t *>(&w);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) q[j] = a[j], q[j + 4] = b[j];
+  for (int i = 0; i < kVec / 4; ++i) {
+    float a[4];
+    four(words[i], a);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[i * 4 + j] = a[j];
+  }
 }
 
 // Scale of a row or of the columns; kInput: the part 2^e of a row's (split_scale), which keeps the values exact in bf16.
-// kVec 8 or 1.  blockDim.x threads a row, blockDim.y rows a block.
+// kVec: 16 bytes of values, or 1.  blockDim.x threads a row, blockDim.y rows a block.
 template <class T, int kVec, bool kByRow, bool kInput = false>
 __device__ __forceinline__ void restore_row(const int8_t *q, int cols, const float *scale, T *x, int first, int step) {
   float s = kByRow ? __ldg(scale) : 0.f;
   if constexpr (kInput) s = split_scale(s).e;
-  if constexpr (kVec == 8) {
+  if constexpr (kVec > 1) {
 #pragma unroll 4
-    for (int c = first * 8; c < cols; c += step * 8) {
-      float v[8];
-      codes8(*reinterpret_cast<const uint2 *>(q + c), v);
+    for (int c = first * kVec; c < cols; c += step * kVec) {
+      float v[kVec];
+      load_codes(q + c, v, [](uint32_t w, float (&a)[4]) { codes4(w, a); });
       if constexpr (kByRow) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= s;
+        for (int j = 0; j < kVec; ++j) v[j] *= s;
       } else if ((reinterpret_cast<uintptr_t>(scale) & 15) == 0) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(scale + c)), b = __ldg(reinterpret_cast<const float4 *>(scale + c) + 1);
-        v[0] *= a.x, v[1] *= a.y, v[2] *= a.z, v[3] *= a.w;
-        v[4] *= b.x, v[5] *= b.y, v[6] *= b.z, v[7] *= b.w;
+#pragma unroll
+        for (int j = 0; j < kVec; j += 4) {
+          const float4 a = __ldg(reinterpret_cast<const float4 *>(scale + c + j));
+          v[j] *= a.x, v[j + 1] *= a.y, v[j + 2] *= a.z, v[j + 3] *= a.w;
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= __ldg(scale + c + j);
+        for (int j = 0; j < kVec; ++j) v[j] *= __ldg(scale + c + j);
       }
-      store8(x + c, v);
+      store_vec(x + c, v);
     }
   } else {
     for (int c = first; c < cols; c += step) x[c] = from_f32<T>(static_cast<float>(q[c]) * (kByRow ? s : __ldg(scale + c)));
@@ -329,14 +370,14 @@ __global__ void __launch_bounds__(256) dequantize_grad(const uint8_t *D, long lo
   grid_dependency_wait();
   const long long stride = static_cast<long long>(gridDim.x) * 256 * kVec;
   for (long long i = (blockIdx.x * 256ll + threadIdx.x) * kVec; i < n; i += stride) {
-    if (kVec == 8 && i + 8 <= n) {
-      const uint2 w = *reinterpret_cast<const uint2 *>(D + i);
-      float a[4], b[4], v[8];
-      grad_steps4(w.x, a);
-      grad_steps4(w.y, b);
+    if (kVec > 1 && i + kVec <= n) {
+      if constexpr (kVec > 1) {
+        float v[kVec];
+        load_codes(D + i, v, [](uint32_t w, float (&a)[4]) { grad_steps4(w, a); });
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = grad_value(a[j]), v[j + 4] = grad_value(b[j]);
-      store8(X + i, v);
+        for (int j = 0; j < kVec; ++j) v[j] = grad_value(v[j]);
+        store_vec(X + i, v);
+      }
     } else {
       for (long long j = i; j < n && j < i + kVec; ++j) {
         float k[4];
@@ -396,20 +437,18 @@ __global__ void __launch_bounds__(256) backward_operands(const __nv_bfloat16 *dC
     for (int r = r0; r < r1; r += 8) {
       const long long i = static_cast<long long>(r) * N + c;
       const uint4 g = *reinterpret_cast<const uint4 *>(dC + i);
-      const uint2 w = *reinterpret_cast<const uint2 *>(D + i);
       const float m = a_scale ? split_scale(__ldg(a_scale + r)).m : 1.f;
-      float a[4], b[4], v[8];
-      grad_steps4(w.x, a);
-      grad_steps4(w.y, b);
+      float k[8], v[8];
+      load_codes(D + i, k, [](uint32_t w, float (&a)[4]) { grad_steps4(w, a); });
       const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float x = __uint_as_float((j & 1) ? gw[j / 2] & 0xFFFF0000u : gw[j / 2] << 16);
-        const float z = x * (j < 4 ? a[j & 3] : b[j & 3]) * (1.f / kGradSteps);
+        const float z = x * k[j] * (1.f / kGradSteps);
         sum[j] += z;
         v[j] = z * m;
       }
-      store8(dz + i, v);
+      store_vec(dz + i, v);
     }
   }
 #pragma unroll
