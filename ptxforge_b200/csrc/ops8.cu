@@ -26,6 +26,7 @@ using pf::DeviceGuard;
 typedef __nv_bfloat16 bf16;
 
 constexpr int kMaxDevices = 64;
+constexpr unsigned long long kWaitNs = 4000000000ull;  // bound of each device-side wait
 constexpr int kMaxSumK = 131071;  // K * 128 * 128 stays below 2^31
 
 // A device's properties and, for each tensor-core kernel that it has launched, the CTA pairs that fit at once (its
@@ -155,33 +156,60 @@ bool vectors_fit(const void *x, long long ld, int cols, int size, int vec) {
 
 template <class T, int kVec>
 void quantize_rows(const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale, cudaStream_t s) {
-  // A warp a row, several rows a block, where its registers hold the row; else a block a row, of as many threads as
-  // the row needs with as few vectors each as 256 threads allow (so that a lone row is spread over a whole SM).
+  // Many rows: a warp each where its registers hold the row, else a block each, eight vectors a thread -- much in flight
+  // and few threads to join.  Few rows: as many threads a row as it can use, so that a lone one is spread over an SM.
+  // Measured, bf16, us: 16384 x 4096 with 2 vectors a thread 52, with 8 HELD8; one row of 4096 HELD1.
   const int vecs = (cols + kVec - 1) / kVec;
   const auto launch = [&](auto kernel, dim3 block) {
     pf::launch_pdl(kernel, dim3(blocks_of(rows, block.y)), block, 0, s, x, ldx, rows, cols, q, ldq, scale);
   };
-  if (vecs <= 64) return launch(&pf::quantize_rows_s8<T, kVec, 2>, dim3(32, 8));
   const auto threads = [&](int held) { return dim3(std::min(512, (vecs + 32 * held - 1) / (32 * held) * 32)); };
+  if (vecs <= 64) return launch(&pf::quantize_rows_s8<T, kVec, 2>, dim3(32, 8));
+  if (rows >= 1024) {
+    if (vecs <= 128) return launch(&pf::quantize_rows_s8<T, kVec, 4>, dim3(32, 8));
+    return launch(&pf::quantize_rows_s8<T, kVec, 8>, vecs <= 256 ? dim3(32, 8) : threads(8));
+  }
   if (vecs <= 512) return launch(&pf::quantize_rows_s8<T, kVec, 2>, threads(2));
   if (vecs <= 1024) return launch(&pf::quantize_rows_s8<T, kVec, 4>, threads(4));
   launch(&pf::quantize_rows_s8<T, kVec, 8>, threads(8));
 }
 
-template <class T, int kVec>
-int quantize_cols(Device &d, const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale,
-                  cudaStream_t s, const Err &err) {
-  // 512 rows of 128 bytes a CTA (three CTAs share an SM, one's loads beside another's stores) as long as 8 CTAs take
-  // them all; above, what an SM's shared memory holds.
-  constexpr int kRowBytes = 128, kMostHeld = 220 * 1024 / kRowBytes;
+// Strips of whole columns held in shared memory: 512 rows of 128 bytes a CTA, so that three CTAs share an SM, one's loads
+// beside another's stores.
+template <class T>
+int quantize_strips(Device &d, const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale,
+                    cudaStream_t s, const Err &err) {
+  constexpr int kRowBytes = 128, kPerCta = pf::kColBox * pf::kColMostBoxes;
   int splits = 1;
-  while (splits < 8 && rows > 512 * splits) splits *= 2;
-  const int share = (rows + splits - 1) / splits, held = std::min(share, kMostHeld);
-  const void *func = reinterpret_cast<const void *>(&pf::quantize_cols_s8<T, kVec>);
+  while (rows > kPerCta * splits) splits *= 2;
+  const int held = ((rows + splits - 1) / splits + pf::kColBox - 1) / pf::kColBox * pf::kColBox;
+  const void *func = reinterpret_cast<const void *>(&pf::quantize_strips_s8<T>);
   int rc, units;
-  if ((rc = kernel_units(d, func, kMostHeld * kRowBytes, 0, err, &units))) return rc;
-  pf::launch_cluster(&pf::quantize_cols_s8<T, kVec>, dim3(blocks_of(static_cast<long long>(cols) * sizeof(T), kRowBytes) * splits),
-                     dim3(256), held * kRowBytes, splits, s, x, ldx, rows, cols, held, q, ldq, scale);
+  if ((rc = kernel_units(d, func, 128 + kPerCta * kRowBytes, 0, err, &units))) return rc;
+  CUtensorMap map;
+  char msg[200];
+  if (pf::encode_2d_msg(msg, sizeof msg, &map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, x,
+                        cols, rows, ldx * sizeof(T), kRowBytes / sizeof(T), pf::kColBox, CU_TENSOR_MAP_SWIZZLE_NONE))
+    return err(PF_ECUDA, "%s", msg);
+  pf::launch_cluster(&pf::quantize_strips_s8<T>, dim3(blocks_of(static_cast<long long>(cols) * sizeof(T), kRowBytes) * splits),
+                     dim3(256), 128 + held * kRowBytes, splits, s, map, rows, cols, q, ldq, scale, d.status, kWaitNs);
+  return PF_OK;
+}
+
+template <class T, int kVec>
+int quantize_cols(const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale, cudaStream_t s,
+                  const Err &err) {
+  uint32_t *amax = reinterpret_cast<uint32_t *>(scale);
+  const cudaError_t e = cudaMemsetAsync(amax, 0, size_t(cols) * sizeof(float), s);
+  if (e != cudaSuccess) return err(PF_ECUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
+  const int col_blocks = static_cast<int>(blocks_of(cols, 32 * kVec));
+  const long long blocks = static_cast<long long>(col_blocks) * blocks_of(rows, pf::kColRows);
+  if (blocks > 0x7FFFFFFF) return err(PF_EINVAL, "more than 2^31 blocks");
+  const dim3 grid(static_cast<unsigned>(blocks));
+  pf::launch_pdl(&pf::amax_cols_s8<T, kVec>, grid, 256, 0, s, x, ldx, rows, cols, col_blocks, amax);
+  pf::launch_pdl(&pf::codes_cols_s8<T, kVec>, grid, 256, 0, s, x, ldx, rows, cols, col_blocks, static_cast<const uint32_t *>(amax),
+                 q, ldq);
+  pf::launch_pdl(&pf::scales_of_bits, dim3(blocks_of(cols, 256)), 256, 0, s, amax, cols);
   return PF_OK;
 }
 
@@ -191,9 +219,11 @@ int quantize(Device &d, const void *X, long long ldx, int rows, int cols, int ax
   constexpr int kVec = 16 / sizeof(T);
   const T *x = static_cast<const T *>(X);
   const bool wide = vectors_fit(X, ldx, cols, sizeof(T), kVec) && vectors_fit(Q, ldq, cols, 1, kVec);
-  if (axis == 0)
-    return wide ? quantize_cols<T, kVec>(d, x, ldx, rows, cols, Q, ldq, scale, s, err)
-                : quantize_cols<T, 1>(d, x, ldx, rows, cols, Q, ldq, scale, s, err);
+  if (axis == 0) {
+    if (wide && rows <= pf::kColMostRows) return quantize_strips<T>(d, x, ldx, rows, cols, Q, ldq, scale, s, err);
+    return wide ? quantize_cols<T, kVec>(x, ldx, rows, cols, Q, ldq, scale, s, err)
+                : quantize_cols<T, 1>(x, ldx, rows, cols, Q, ldq, scale, s, err);
+  }
   if (wide) quantize_rows<T, kVec>(x, ldx, rows, cols, Q, ldq, scale, s);
   else quantize_rows<T, 1>(x, ldx, rows, cols, Q, ldq, scale, s);
   return PF_OK;
@@ -292,7 +322,6 @@ int operand_maps(const Product &g, const Err &err, CUtensorMap *w, CUtensorMap *
   return PF_OK;
 }
 
-constexpr unsigned long long kWaitNs = 4000000000ull;
 constexpr int kSmemPerSm = 227 * 1024;  // of one SM, for the CTAs that share it
 constexpr int kOneStatic = 3072;        // of gemm8_one: barriers and token scalars
 

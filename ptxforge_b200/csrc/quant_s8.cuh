@@ -136,11 +136,38 @@ struct Largest<__nv_bfloat16, 8> {
   }
 };
 
+// The same, a column each.
+template <class T, int kVec>
+struct ColumnLargest {
+  uint32_t m[kVec] = {};
+  __device__ __forceinline__ void take(const Values<T, kVec> &x) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) m[j] = max(m[j], abs_bits(x[j]));
+  }
+  __device__ __forceinline__ uint32_t bits(int j) const { return m[j]; }
+};
+template <>
+struct ColumnLargest<__nv_bfloat16, 8> {
+  __nv_bfloat162 m[4];
+  __device__ __forceinline__ ColumnLargest() {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = __floats2bfloat162_rn(0.f, 0.f);
+  }
+  __device__ __forceinline__ void take(const Values<__nv_bfloat16, 8> &x) {
+    const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&x.w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = __hmax2_nan(m[j], __habs2(p[j]));
+  }
+  __device__ __forceinline__ uint32_t bits(int j) const {
+    return abs_bits(j & 1 ? __high2float(m[j / 2]) : __low2float(m[j / 2]));
+  }
+};
+
 // Codes of kVec values with the scales s[j] (one for all where kOne).  1.5 2^23 + x / s holds the code in its low byte,
 // rounded to the nearest whole number by the addition; vectors with a value near a half step are done again by
-// code_of.  A scale that is NaN gives code 0.
+// code_of, as are those with a scale that is NaN (`bad`), whose codes are 0.
 template <class T, int kVec, bool kOne>
-__device__ __forceinline__ void store_codes(const Values<T, kVec> &x, const float *s, const float *inv, int8_t *q) {
+__device__ __forceinline__ void store_codes(const Values<T, kVec> &x, const float *s, const float *inv, bool bad, int8_t *q) {
   constexpr float magic = 12582912.f;
   uint32_t r[kVec];
   float far = 0.f;
@@ -161,14 +188,7 @@ __device__ __forceinline__ void store_codes(const Values<T, kVec> &x, const floa
       r[j + 1] = __float_as_uint(y.y);
     }
   }
-  bool again = far > 0.5f - 3e-5f;
-  if constexpr (kOne) {
-    again |= s[0] != s[0];
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) again |= s[j] != s[j];
-  }
-  if (again) {
+  if (bad || far > 0.5f - 3e-5f) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) r[j] = static_cast<uint32_t>(code_of(x[j], s[kOne ? 0 : j], inv[kOne ? 0 : j]));
   }
@@ -226,12 +246,12 @@ __global__ void __launch_bounds__(512) quantize_rows_s8(const T *X, long long ld
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     const int v = threadIdx.x + i * step;
-    if (v < vecs) store_codes<T, kVec, true>(held[i], &s, &inv, q + static_cast<long long>(v) * kVec);
+    if (v < vecs) store_codes<T, kVec, true>(held[i], &s, &inv, s != s, q + static_cast<long long>(v) * kVec);
   }
   for (int v = threadIdx.x + kHeld * step; v < vecs; v += step) {
     Values<T, kVec> y;
     y.load(x + static_cast<long long>(v) * kVec);
-    store_codes<T, kVec, true>(y, &s, &inv, q + static_cast<long long>(v) * kVec);
+    store_codes<T, kVec, true>(y, &s, &inv, s != s, q + static_cast<long long>(v) * kVec);
   }
   if (threadIdx.x == 0) scale[r] = s;
 }
@@ -239,66 +259,161 @@ __global__ void __launch_bounds__(512) quantize_rows_s8(const T *X, long long ld
 // ------------------------------------------------------------------------------------------------
 // a scale for each column
 // ------------------------------------------------------------------------------------------------
-// A cluster takes a strip of 128 bytes of columns, each of its CTAs a share of the rows, of which it holds `held` in
-// shared memory: one pass over X.  The column maxima are joined through distributed shared memory.  What a longer share
-// has beyond the held rows is read again.
-template <class T, int kVec>
-__global__ void __launch_bounds__(256) quantize_cols_s8(const T *X, long long ldx, int rows, int cols, int held, int8_t *Q,
-                                                        long long ldq, float *scale) {
-  constexpr int W = 128 / sizeof(T), LANES = W / kVec, STEP = 256 / LANES;  // columns; threads a row; rows at once
+// Up to 4096 aligned rows: a cluster takes a strip of 128 bytes of columns, each of its CTAs a share of the rows, which
+// comes to shared memory by TMA, all boxes on their way at once, and stays there: one pass over X.  The column maxima are
+// joined through distributed shared memory.
+constexpr int kColBox = 64, kColMostBoxes = 8, kColMostRows = 8 * kColBox * kColMostBoxes;
+template <class T>
+__global__ void __launch_bounds__(256, 3) quantize_strips_s8(const __grid_constant__ CUtensorMap map, int rows, int cols,
+                                                             int8_t *Q, long long ldq, float *scale, unsigned *status,
+                                                             unsigned long long timeout_ns) {
+  constexpr int kVec = 16 / sizeof(T), W = 128 / sizeof(T), LANES = W / kVec, STEP = 256 / LANES;  // LANES = 8, STEP = 32
   typedef Values<T, kVec> Vec;
-  extern __shared__ uint4 slab4[];
-  T *slab = reinterpret_cast<T *>(slab4);
+  extern __shared__ uint8_t smem_raw[];
+  T *slab = reinterpret_cast<T *>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
   __shared__ uint32_t amax[W];
+  __shared__ float scales[2][W];
+  __shared__ uint64_t full[kColMostBoxes];
+  __shared__ int abort_word;
   uint32_t splits;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
   const int rank = static_cast<int>(cluster_ctarank());
-  const long long r0 = static_cast<long long>(rows) * rank / splits, r1 = static_cast<long long>(rows) * (rank + 1) / splits;
-  const int n = static_cast<int>(r1 - r0);
+  const int r0 = rows * rank / static_cast<int>(splits), n = rows * (rank + 1) / static_cast<int>(splits) - r0;
   const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES;
-  const long long c = static_cast<long long>(blockIdx.x / splits) * W + lane * kVec;
-  const bool inside = c < cols;  // whole vectors: cols is a multiple of kVec
-  const T *x = X + r0 * ldx + c;
+  const int c0 = static_cast<int>(blockIdx.x / splits) * W, c = c0 + lane * kVec;
+  const int boxes = (n + kColBox - 1) / kColBox;
   grid_launch_dependents();
-  grid_dependency_wait();
   if (threadIdx.x < W) amax[threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map);
+    for (int b = 0; b < boxes; ++b) mbar_init(&full[b], 1);
+    abort_word = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  grid_dependency_wait();
   __syncthreads();
-  uint32_t m[kVec] = {};
-  if (inside) {
-#pragma unroll 8
-    for (int r = first; r < n; r += STEP) {
-      Vec y;
-      y.load(x + r * ldx);
-      if (r < held) *reinterpret_cast<decltype(y.w) *>(slab + r * W + lane * kVec) = y.w;
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) m[j] = max(m[j], abs_bits(y[j]));
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < boxes; ++b) {
+      mbar_arrive_expect_tx(&full[b], kColBox * 128);
+      tma_load_2d(slab + b * kColBox * W, &map, &full[b], c0, r0 + b * kColBox);
+    }
+  }
+  ColumnLargest<T, kVec> largest;
+  for (int b = 0; b < boxes; ++b) {
+    if (!mbar_wait(&full[b], 0, timeout_ns, &abort_word)) {
+      atomicOr(status, 1u);
+      abort_word = 1;
     }
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) atomicMax(&amax[lane * kVec + j], m[j]);
+    for (int k = 0; k < kColBox / STEP; ++k) {
+      const int r = b * kColBox + k * STEP + first;
+      Vec y;
+      y.load(slab + r * W + lane * kVec);
+      if (r < n) largest.take(y);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    // the lanes of a warp that hold the same columns first, then one of them for the warp
+    uint32_t m = largest.bits(j);
+#pragma unroll
+    for (int d = LANES; d < 32; d *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if ((threadIdx.x & 31) < LANES) atomicMax(&amax[lane * kVec + j], m);
   }
   __syncwarp();
   cluster_sync();
-  if (inside) {
+  // a thread a column: every CTA's maximum, all loads on their way at once
+  if (threadIdx.x < W) {
+    uint32_t all = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k)
+      if (k < splits) all = max(all, ld_cluster(mapa_shared(smem_u32(&amax[threadIdx.x]), k)));
+    const float s = scale_of(all);
+    scales[0][threadIdx.x] = s;
+    scales[1][threadIdx.x] = __fdiv_rn(1.f, s);
+    if (rank == 0 && c0 + static_cast<int>(threadIdx.x) < cols) scale[c0 + threadIdx.x] = s;
+  }
+  __syncthreads();
+  if (c < cols) {  // whole vectors: cols is a multiple of kVec
     float s[kVec], inv[kVec];
+    bool bad = false;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      uint32_t all = 0;
-      for (uint32_t k = 0; k < splits; ++k) all = max(all, ld_cluster(mapa_shared(smem_u32(&amax[lane * kVec + j]), k)));
-      s[j] = scale_of(all);
-      inv[j] = __fdiv_rn(1.f, s[j]);
-      if (rank == 0 && first == 0) scale[c + j] = s[j];
+      s[j] = scales[0][lane * kVec + j], inv[j] = scales[1][lane * kVec + j];
+      bad |= s[j] != s[j];
     }
     int8_t *q = Q + r0 * ldq + c;
 #pragma unroll 4
     for (int r = first; r < n; r += STEP) {
       Vec y;
-      if (r < held) y.w = *reinterpret_cast<const decltype(y.w) *>(slab + r * W + lane * kVec);
-      else y.load(x + r * ldx);
-      store_codes<T, kVec, false>(y, s, inv, q + r * ldq);
+      y.load(slab + r * W + lane * kVec);
+      store_codes<T, kVec, false>(y, s, inv, bad, q + r * ldq);
     }
   }
   __syncwarp();
   cluster_sync();  // nobody leaves while its maxima may be read
+}
+
+// Any matrix, two passes: 32 vectors of columns x kColRows rows a block.  First the largest abs_bits of each column into
+// `scale` (zeroed before; a maximum of bits does not depend on the order), then the codes, then the scales over the bits.
+constexpr int kColRows = 128;
+template <class T, int kVec>
+__global__ void __launch_bounds__(256) amax_cols_s8(const T *X, long long ldx, int rows, int cols, int col_blocks, uint32_t *amax) {
+  __shared__ uint32_t sh[8][32 * kVec];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int rb = blockIdx.x / col_blocks, c0 = (blockIdx.x - rb * col_blocks) * 32 * kVec, c = c0 + lane * kVec;
+  const int r1 = min(static_cast<long long>(rows), (rb + 1ll) * kColRows);
+  ColumnLargest<T, kVec> largest;
+  if (c < cols) {
+#pragma unroll 8
+    for (int r = rb * kColRows + row; r < r1; r += 8) {
+      Values<T, kVec> y;
+      y.load(X + r * ldx + c);
+      largest.take(y);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) sh[row][lane * kVec + j] = largest.bits(j);
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * kVec; i += 256)
+    if (c0 + i < cols) {
+      uint32_t all = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) all = max(all, sh[k][i]);
+      atomicMax(amax + c0 + i, all);
+    }
+}
+template <class T, int kVec>
+__global__ void __launch_bounds__(256) codes_cols_s8(const T *X, long long ldx, int rows, int cols, int col_blocks,
+                                                     const uint32_t *amax, int8_t *Q, long long ldq) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int rb = blockIdx.x / col_blocks, c = ((blockIdx.x - rb * col_blocks) * 32 + lane) * kVec;
+  if (c >= cols) return;
+  const int r1 = min(static_cast<long long>(rows), (rb + 1ll) * kColRows);
+  float s[kVec], inv[kVec];
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    s[j] = scale_of(__ldg(amax + c + j)), inv[j] = __fdiv_rn(1.f, s[j]);
+    bad |= s[j] != s[j];
+  }
+#pragma unroll 4
+  for (int r = rb * kColRows + row; r < r1; r += 8) {
+    Values<T, kVec> y;
+    y.load(X + r * ldx + c);
+    store_codes<T, kVec, false>(y, s, inv, bad, Q + r * ldq + c);
+  }
+}
+__global__ void __launch_bounds__(256) scales_of_bits(uint32_t *amax, int n) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) amax[i] = __float_as_uint(scale_of(amax[i]));
 }
 
 // ------------------------------------------------------------------------------------------------
