@@ -70,13 +70,14 @@ struct Gemm8Params {
   int channels, tokens;          // out's columns and rows
   int c_tiles, t_tiles, k_blocks;
   int group;                     // gemm8_pair: channel tiles that the raster walks before the next token tile
+  int tiles;                     // gemm8_pair: the first so many of them
   int stages;                    // gemm8_one: pipeline depth, by the shared memory given
   unsigned *status;
   unsigned long long timeout_ns;
 };
 
 // ------------------------------------------------------------------------------------------------
-// epilogues: one object a lane, for its channel
+// epilogues: one object a lane, for its channel.  Args::part: those of the product's part from channel c0, token t0 on.
 // ------------------------------------------------------------------------------------------------
 template <class Out>
 struct EpilogueS8 {
@@ -85,6 +86,7 @@ struct EpilogueS8 {
     Out *out;
     long long ld;
     int gelu;
+    Args part(int c0, int t0) const { return {sa + t0, sb + c0, bias ? bias + c0 : nullptr, out + t0 * ld + c0, ld, gelu}; }
   };
   static constexpr bool kTokenScalar = true;
   const Args &a;
@@ -139,6 +141,7 @@ struct EpilogueCheckpoint : EpilogueF32Sum {
     __nv_bfloat16 *out;
     uint8_t *codes;
     long long ld;
+    Args part(int c0, int t0) const { return {bias + c0, out + t0 * ld + c0, codes + t0 * ld + c0, ld}; }
   };
   static constexpr bool kTokenScalar = false;
   const Args &a;
@@ -183,6 +186,7 @@ struct EpilogueBf16 : EpilogueF32Sum {
     const float *token_scale;
     __nv_bfloat16 *out;
     long long ld;
+    Args part(int c0, int t0) const { return {token_scale ? token_scale + t0 : nullptr, out + t0 * ld + c0, ld}; }
   };
   static constexpr bool kTokenScalar = kDivided;
   const Args &a;
@@ -454,7 +458,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int tiles = p.c_tiles * p.t_tiles;
+  const int tiles = p.tiles;
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmW);

@@ -303,6 +303,13 @@ struct Product {
   int tokens, channels, sum;
   const void *T, *W;
   long long ldt, ldw;
+  // The part from channel c0, token t0 on.
+  template <class Op>
+  Product part(int c0, int t0) const {
+    return {tokens - t0, channels - c0, sum,
+            static_cast<const char *>(T) + (Op::T_K ? t0 * ldt : t0) * Op::ELEM,
+            static_cast<const char *>(W) + (Op::W_K ? c0 * ldw : c0) * Op::ELEM, ldt, ldw};
+  }
 };
 
 template <int kElem>
@@ -353,7 +360,10 @@ int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStr
   return launched(err);
 }
 
-template <class Op, class Epi, int kStages>
+// Whole waves of 256 x 256 tiles by the pair kernel.  Where the last wave would leave more than half of the pairs idle, its
+// tiles (a rectangle: the last token columns of the raster's last group) go to the one-CTA kernel, which spreads them
+// over the whole GPU: dB of 4096 x 14336 x 8192, 896 tiles on 74 pairs, TAIL.
+template <class Op, class One, class Epi, int kStages>
 int run_pair(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
   using Cfg = pf::PairConfig<Op, kStages>;
   CUtensorMap w, t;
@@ -372,9 +382,15 @@ int run_pair(Device &d, const Product &g, const typename Epi::Args &args, cudaSt
   p.timeout_ns = kWaitNs;
   const long long tiles = static_cast<long long>(p.c_tiles) * p.t_tiles;
   if (tiles > (1ll << 30)) return err(PF_EINVAL, "more than 2^30 tiles of 256 x 256");
-  pf::launch_pdl(&pf::gemm8_pair<Op, Epi, kStages>, dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, units))),
-                 Cfg::THREADS, Cfg::SMEM_BYTES, s, w, t, p, args);
-  return launched(err);
+  const int last = static_cast<int>(tiles % units), rows = p.c_tiles - (p.c_tiles - 1) / p.group * p.group;
+  int columns = (last + rows - 1) / rows;
+  if (tiles < units || 2 * columns * rows > units || columns >= p.t_tiles) columns = 0;
+  p.tiles = static_cast<int>(tiles) - columns * rows;
+  pf::launch_pdl(&pf::gemm8_pair<Op, Epi, kStages>, dim3(2 * std::min(p.tiles, units)), Cfg::THREADS, Cfg::SMEM_BYTES, s, w, t, p,
+                 args);
+  if ((rc = launched(err)) || columns == 0) return rc;
+  const int c0 = (p.c_tiles - rows) * 256, t0 = (p.t_tiles - columns) * 256;
+  return run_one<One, Epi>(d, g.part<One>(c0, t0), args.part(c0, t0), s, err);
 }
 
 // Elements, W's and T's order, epilogue -> the kernel for the sizes.
@@ -383,7 +399,7 @@ int product(Device &d, const Product &g, const typename Epi::Args &args, cudaStr
   using pf::Operands;
   const long long pair_tiles = ((g.channels + 255ll) / 256) * ((g.tokens + 255ll) / 256);
   if (g.tokens > 128 && pair_tiles >= 32)
-    return run_pair<Operands<kElem, kWK, kTK, 128, 2>, Epi, 3>(d, g, args, s, err);
+    return run_pair<Operands<kElem, kWK, kTK, 128, 2>, Operands<kElem, kWK, kTK, 128, 1>, Epi, 3>(d, g, args, s, err);
   if constexpr (kTK) {
     if (g.tokens <= 16) return run_one<Operands<kElem, kWK, kTK, 16, 1>, Epi>(d, g, args, s, err);
     if (g.tokens <= 32) return run_one<Operands<kElem, kWK, kTK, 32, 1>, Epi>(d, g, args, s, err);
