@@ -79,6 +79,31 @@ struct Gemm8Params {
 // ------------------------------------------------------------------------------------------------
 // epilogues: one object a lane, for its channel.  Args::part: those of the product's part from channel c0, token t0 on.
 // ------------------------------------------------------------------------------------------------
+// Four neighbouring channels of a token, as the split sums come back (join_sums): `n` of them exist; `whole`: rows start
+// on four-value boundaries, so that one store writes them.
+__device__ __forceinline__ void store4(float *out, const float4 &y) { *reinterpret_cast<float4 *>(out) = y; }
+__device__ __forceinline__ void store4(__nv_bfloat16 *out, const float4 &y) {
+  *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+}
+template <class Out>
+__device__ __forceinline__ void store_channels(Out *out, const float4 &y, int n, bool whole) {
+  if (whole && n >= 4) {
+    store4(out, y);
+  } else {
+    const float v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) out[j] = from_f32<Out>(v[j]);
+  }
+}
+template <class Out>
+__device__ __forceinline__ bool rows_of_four(const Out *out, long long ld) {
+  return ld % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(Out)) == 0;
+}
+__device__ __forceinline__ float4 load_channels(const float *p, int n) {
+  return make_float4(n > 0 ? __ldg(p) : 0.f, n > 1 ? __ldg(p + 1) : 0.f, n > 2 ? __ldg(p + 2) : 0.f, n > 3 ? __ldg(p + 3) : 0.f);
+}
+
 template <class Out>
 struct EpilogueS8 {
   struct Args {
@@ -111,11 +136,11 @@ struct EpilogueS8 {
     const float2 y = a.gelu ? value<true>(sum, sum, sa, sa) : value<false>(sum, sum, sa, sa);
     if (inside) a.out[t * a.ld + c] = from_f32<Out>(y.x);
   }
-  template <bool kGelu>
-  __device__ __forceinline__ void put32_as(const uint32_t (&v)[32], int t0, const float *scalars) const {
+  template <bool kGelu, int N>
+  __device__ __forceinline__ void put_as(const uint32_t (&v)[N], int t0, const float *scalars) const {
     Out *out = a.out + t0 * a.ld + c;
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
+    for (int j = 0; j < N; j += 2) {
       const float2 y = value<kGelu>(v[j], v[j + 1], scalars[j], scalars[j + 1]);
       if (inside) {
         out[j * a.ld] = from_f32<Out>(y.x);
@@ -123,10 +148,31 @@ struct EpilogueS8 {
       }
     }
   }
-  __device__ __forceinline__ void put32(const uint32_t (&v)[32], int t0, const float *scalars) const {
-    if (a.gelu) put32_as<true>(v, t0, scalars);
-    else put32_as<false>(v, t0, scalars);
+  template <int N>
+  __device__ __forceinline__ void put_all(const uint32_t (&v)[N], int t0, const float *scalars) const {
+    if (a.gelu) put_as<true>(v, t0, scalars);
+    else put_as<false>(v, t0, scalars);
   }
+  struct Row {
+    const Args &a;
+    const int c, n;
+    const bool whole;
+    float4 sb, bias;
+    __device__ __forceinline__ Row(const Args &args, int c0, int channels)
+        : a(args), c(c0), n(channels - c0), whole(rows_of_four(args.out, args.ld)) {
+      sb = load_channels(a.sb + c, n);
+      bias = a.bias ? load_channels(a.bias + c, n) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __device__ __forceinline__ void put(const uint32_t (&v)[4], int t, float sa) const {
+      const auto two = [&](uint32_t v0, uint32_t v1, float s0, float s1, float b0, float b1) {
+        const float2 x = __ffma2_rn(make_float2(static_cast<float>(static_cast<int>(v0)), static_cast<float>(static_cast<int>(v1))),
+                                    __fmul2_rn(both(sa), make_float2(s0, s1)), make_float2(b0, b1));
+        return a.gelu ? gelu_of(x) : x;
+      };
+      const float2 y0 = two(v[0], v[1], sb.x, sb.y, bias.x, bias.y), y1 = two(v[2], v[3], sb.z, sb.w, bias.z, bias.w);
+      store_channels(a.out + t * a.ld + c, make_float4(y0.x, y0.y, y1.x, y1.y), n, whole);
+    }
+  };
 };
 
 struct EpilogueF32Sum {
@@ -161,12 +207,13 @@ struct EpilogueCheckpoint : EpilogueF32Sum {
       a.codes[t * a.ld + c] = static_cast<uint8_t>(grad_codes(g.d).x);
     }
   }
-  __device__ __forceinline__ void put32(const uint32_t (&v)[32], int t0, const float *) const {
+  template <int N>
+  __device__ __forceinline__ void put_all(const uint32_t (&v)[N], int t0, const float *) const {
     const long long i = t0 * a.ld + c;
     __nv_bfloat16 *out = a.out + i;
     uint8_t *codes = a.codes + i;
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
+    for (int j = 0; j < N; j += 2) {
       const Gelu2 g = gelu_and_grad(__fadd2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), both(bias)));
       const uint2 code = grad_codes(g.d);
       if (inside) {
@@ -177,6 +224,25 @@ struct EpilogueCheckpoint : EpilogueF32Sum {
       }
     }
   }
+  struct Row {  // channels come in eights here
+    const Args &a;
+    const int c;
+    const bool inside;
+    float4 bias;
+    __device__ __forceinline__ Row(const Args &args, int c0, int channels) : a(args), c(c0), inside(c0 < channels) {
+      bias = load_channels(a.bias + c, channels - c0);
+    }
+    __device__ __forceinline__ void put(const uint32_t (&v)[4], int t, float) const {
+      const Gelu2 g0 = gelu_and_grad(make_float2(__uint_as_float(v[0]) + bias.x, __uint_as_float(v[1]) + bias.y));
+      const Gelu2 g1 = gelu_and_grad(make_float2(__uint_as_float(v[2]) + bias.z, __uint_as_float(v[3]) + bias.w));
+      const uint2 k0 = grad_codes(g0.d), k1 = grad_codes(g1.d);
+      if (!inside) return;
+      const long long i = t * a.ld + c;
+      store4(a.out + i, make_float4(g0.y.x, g0.y.y, g1.y.x, g1.y.y));
+      *reinterpret_cast<uint32_t *>(a.codes + i) =
+          __byte_perm(__byte_perm(k0.x, k0.y, 0x0040), __byte_perm(k1.x, k1.y, 0x0040), 0x5410);
+    }
+  };
 };
 
 // kDivided: a token's row is divided by its m (split_scale of its input scale).
@@ -200,14 +266,27 @@ struct EpilogueBf16 : EpilogueF32Sum {
   __device__ __forceinline__ void put(uint32_t sum, int t, float inv_m) const {
     if (inside) a.out[t * a.ld + c] = __float2bfloat16_rn(__uint_as_float(sum) * (kDivided ? inv_m : 1.f));
   }
-  __device__ __forceinline__ void put32(const uint32_t (&v)[32], int t0, const float *scalars) const {
+  template <int N>
+  __device__ __forceinline__ void put_all(const uint32_t (&v)[N], int t0, const float *scalars) const {
     __nv_bfloat16 *out = a.out + t0 * a.ld + c;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
+    for (int j = 0; j < N; ++j) {
       const __nv_bfloat16 y = __float2bfloat16_rn(__uint_as_float(v[j]) * (kDivided ? scalars[j] : 1.f));
       if (inside) out[j * a.ld] = y;
     }
   }
+  struct Row {  // channels come in eights here
+    const Args &a;
+    const int c;
+    const bool inside;
+    __device__ __forceinline__ Row(const Args &args, int c0, int channels) : a(args), c(c0), inside(c0 < channels) {}
+    __device__ __forceinline__ void put(const uint32_t (&v)[4], int t, float inv_m) const {
+      const float f = kDivided ? inv_m : 1.f;
+      if (inside)
+        store4(a.out + t * a.ld + c, make_float4(__uint_as_float(v[0]) * f, __uint_as_float(v[1]) * f, __uint_as_float(v[2]) * f,
+                                                 __uint_as_float(v[3]) * f));
+    }
+  };
 };
 
 // The scalars of tokens [t0, t0 + 32 n) into this warp's shared memory, from which a broadcast load brings four.
@@ -224,15 +303,15 @@ __device__ __forceinline__ void stage_scalars(const typename Epi::Args &args, in
   }
 }
 
-// 32 tokens from t0 on.  Whole blocks run without a branch a token, so that the arithmetic of many overlaps (with one, a
+// N tokens from t0 on.  Whole blocks run without a branch a token, so that the arithmetic of many overlaps (with one, a
 // tile of 256 x 256 took 27 us).
-template <class Epi>
-__device__ __forceinline__ void put32(const Epi &e, const uint32_t (&v)[32], int t0, int tokens, const float *scalars) {
-  if (t0 + 32 <= tokens) {
-    e.put32(v, t0, scalars);
+template <class Epi, int N>
+__device__ __forceinline__ void put_block(const Epi &e, const uint32_t (&v)[N], int t0, int tokens, const float *scalars) {
+  if (t0 + N <= tokens) {
+    e.put_all(v, t0, scalars);
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < N; ++j)
       if (t0 + j < tokens) e.put(v[j], t0 + j, Epi::kTokenScalar ? scalars[j] : 0.f);
   }
 }
@@ -243,8 +322,40 @@ __device__ __forceinline__ void put32(const Epi &e, const uint32_t (&v)[32], int
 constexpr int kOneThreads = 192;
 constexpr int kOneMaxStages = 16;
 
+// This CTA's share of the tokens: every CTA's sums, added in rank order.  They lie as [token][128 channels]; a warp takes a
+// token, a lane four of its channels, so that what crosses between SMs are whole lines (as [channel][token], 16 bytes a
+// lane, eight CTAs' sums of 128 x 128 took 50 us), and the sums of several tokens are on their way before the first
+// addition.
+template <int kTokens, int kSplits, class Epi>
+__device__ __forceinline__ void join_sums(const typename Epi::Args &args, int c0, int channels, uint32_t base, uint32_t rank,
+                                          int warp, int lane, int t0, int tokens, const float *scalars) {
+  constexpr int SHARE = kTokens / kSplits, AHEAD = SHARE < 4 ? 1 : kSplits == 8 || SHARE < 16 ? 1 : kSplits == 4 ? 2 : 4;
+  const typename Epi::Row row(args, c0 + lane * 4, channels);
+  const int mine = static_cast<int>(rank) * SHARE;
+  uint32_t from[kSplits];
+#pragma unroll
+  for (int s = 0; s < kSplits; ++s) from[s] = mapa_shared(base + lane * 16, s);
+#pragma unroll 1
+  for (int t = mine + warp; t < mine + SHARE && t0 + t < tokens; t += 4 * AHEAD) {
+    uint32_t v[AHEAD][kSplits][4];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+      for (int s = 0; s < kSplits; ++s) ld_cluster<4>(from[s] + (t + i * 4) * 512, v[i][s]);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+#pragma unroll
+      for (int s = 1; s < kSplits; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][0][j] = Epi::add(v[i][0][j], v[i][s][j]);
+      const int at = t + i * 4;
+      if (t0 + at < tokens) row.put(v[i][0], t0 + at, Epi::kTokenScalar ? scalars[at] : 0.f);
+    }
+  }
+}
+
 template <class Op, class Epi>
-__global__ void __launch_bounds__(kOneThreads)
+__global__ void __launch_bounds__(kOneThreads, 4)
     gemm8_one(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const Gemm8Params p,
               const typename Epi::Args args) {
   constexpr int TOKENS = Op::TOKENS;
@@ -264,6 +375,7 @@ __global__ void __launch_bounds__(kOneThreads)
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
   const uint32_t rank = cluster_ctarank();
   const int c0 = static_cast<int>(blockIdx.x / splits) * 128, t0 = static_cast<int>(blockIdx.y) * TOKENS;
+  const int tokens = min(p.tokens, t0 + TOKENS);
   // this CTA's share of the sum
   const int kb0 = static_cast<int>(static_cast<long long>(p.k_blocks) * rank / splits);
   const int kb1 = static_cast<int>(static_cast<long long>(p.k_blocks) * (rank + 1) / splits);
@@ -363,25 +475,25 @@ __global__ void __launch_bounds__(kOneThreads)
     const int c_local = q * 32 + lane;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const Epi epi(args, c0 + c_local, p.channels);
-    if (splits == 1) stage_scalars<Epi>(args, t0, (TOKENS + 31) / 32, p.tokens, lane, scalars[q]);
+    stage_scalars<Epi>(args, t0, (TOKENS + 31) / 32, tokens, lane, scalars[q]);
     const bool waited = mbar_wait(&done, 0, p.timeout_ns, abort_flag);
     if (!__all_sync(0xffffffffu, waited)) {
       if (lane == 0) fail(kErrEpilogueWait);
     } else {
       tc_fence_after();
+      constexpr int N = TOKENS < 32 ? TOKENS : 32;
       uint32_t *mine = reinterpret_cast<uint32_t *>(smem) + c_local;  // [token][128 channels], where the stages were
 #pragma unroll 1
-      for (int b = 0; b < (TOKENS + 31) / 32; ++b) {
-        if (t0 + b * 32 >= p.tokens) break;
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(t_row + b * 32, v);
+      for (int b = 0; b < TOKENS / N; ++b) {
+        if (t0 + b * N >= tokens) break;
+        uint32_t v[N];
+        tmem_ld<N>(t_row + b * N, v);
         tmem_ld_wait();
         if (splits == 1) {
-          put32(epi, v, t0 + b * 32, min(p.tokens, t0 + TOKENS), scalars[q] + b * 32);
+          put_block(epi, v, t0 + b * N, tokens, scalars[q] + b * N);
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (b * 32 + j < TOKENS) mine[(b * 32 + j) * 128] = v[j];
+          for (int j = 0; j < N; ++j) mine[(b * N + j) * 128] = v[j];
         }
       }
     }
@@ -390,15 +502,11 @@ __global__ void __launch_bounds__(kOneThreads)
     __syncwarp();
     cluster_sync();  // every CTA's sums are in its shared memory
     if (warp >= 2) {
-      const int c_local = (warp & 3) * 32 + lane;
-      const Epi epi(args, c0 + c_local, p.channels);
-      const uint32_t base = smem_u32(smem) + c_local * 4;
-      const int n = min(TOKENS, p.tokens - t0);
-      for (int t = static_cast<int>(rank); t < n; t += static_cast<int>(splits)) {
-        uint32_t sum = ld_cluster(mapa_shared(base + t * 512, 0));
-        for (uint32_t s = 1; s < splits; ++s) sum = Epi::add(sum, ld_cluster(mapa_shared(base + t * 512, s)));
-        epi.put(sum, t0 + t, Epi::token(args, t0 + t));
-      }
+      const uint32_t base = smem_u32(smem);
+      const float *sc = scalars[warp & 3];
+      if (splits == 2) join_sums<TOKENS, 2, Epi>(args, c0, p.channels, base, rank, warp - 2, lane, t0, tokens, sc);
+      else if (splits == 4) join_sums<TOKENS, 4, Epi>(args, c0, p.channels, base, rank, warp - 2, lane, t0, tokens, sc);
+      else join_sums<TOKENS, 8, Epi>(args, c0, p.channels, base, rank, warp - 2, lane, t0, tokens, sc);
     }
     __syncwarp();
     cluster_sync();  // nobody leaves while its shared memory may be read
@@ -613,7 +721,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
         }
-        if (t0 + b * 32 < p.tokens) put32(epi, v[b & 1], t0 + b * 32, p.tokens, mine + b * 32);
+        if (t0 + b * 32 < p.tokens) put_block(epi, v[b & 1], t0 + b * 32, p.tokens, mine + b * 32);
       }
       if (++acc == 2) {
         acc = 0;

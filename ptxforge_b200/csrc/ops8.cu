@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -332,8 +333,45 @@ int operand_maps(const Product &g, const Err &err, CUtensorMap *w, CUtensorMap *
 constexpr int kSmemPerSm = 227 * 1024;  // of one SM, for the CTAs that share it
 constexpr int kOneStatic = 3072;        // of gemm8_one: barriers and token scalars
 
+// What a product costs, in us on a B200, by the measurements below; it is used to choose a kernel, never to skip work.
+//   one CTA, T tokens a tile, S splits: an SM takes in 92 KB/us of operands with one CTA, 130 with more (a k-block is 16 KB
+//   of W and T / 8 KB of T), or all of them W from HBM at 6.7 GB/ms; 3.5 for the launch, T / 40 for T tokens' epilogue
+//   (with splits 0.7 + T / 125 for the exchange and a share of that); CTAs that do not fit at once start 3 later.
+//   pair: 0.28 a k-block and wave, 11.5 for the launch and the last epilogue.
+// Measured / by this rule, bf16, M x N x K: 1024 x 2048 x 8192 T128 S2 36 / 38, S1 50 / 51, pair 49 / 47;
+// 512 x 4096 x 4096 T128 S2 23 / 23, pair 30 / 29; 256 x 4096 x 4096 T128 S4 16 / 15, T64 S2 17 / 17; 1024^3 T64 S2 9.4 / 9.4;
+// 2048^3 pair 21 / 20, T128 S1 24 / 24.
+struct Choice {
+  int tokens = 0, splits = 1;
+  double us = 1e30;
+};
+int k_blocks_of(int sum, int elem) { return (sum + 128 / elem - 1) / (128 / elem); }
+Choice choose_one(const Device &d, int tokens, int channels, int sum, int elem, int least_tokens) {
+  Choice best;
+  const int kb = k_blocks_of(sum, elem);
+  const double hbm = double(channels) * sum * elem / 6.7e6;
+  for (int T = least_tokens; T <= 128; T *= 2) {
+    const double tiles = std::ceil(channels / 128.0) * std::ceil(tokens / double(T));
+    for (int S = 1; S <= 8 && kb >= 2 * S - 1; S *= 2) {
+      const double ctas = std::ceil(tiles * S / d.num_sms), blocks = (kb + S - 1) / S;
+      const double in = ctas * blocks * (16 + T / 8) / (ctas > 1 ? 130 : 92);
+      const double epilogue = S == 1 ? T / 40.0 : 0.7 + T / 125.0 + T / (40.0 * S);
+      const double late = std::ceil(ctas / (T <= 64 ? 3 : 2)) - 1;
+      const double us = 3.5 + std::max(in, hbm) + epilogue * (1 + 0.5 * std::min(ctas - 1, 2.0)) + 3 * late;
+      if (us < best.us) best = {T, S, us};
+    }
+  }
+  return best;
+}
+double pair_us(const Device &d, int tokens, int channels, int sum, int elem) {
+  const double tiles = std::ceil(channels / 256.0) * std::ceil(tokens / 256.0), waves = tiles / (d.num_sms / 2);
+  // a short last wave goes to the one-CTA kernel (run_pair): about half a wave and a launch
+  const double part = waves - std::floor(waves), whole = waves > 1 && part > 0 && part <= 0.5 ? std::floor(waves) + 0.5 : std::ceil(waves);
+  return 11.5 + 0.28 * whole * k_blocks_of(sum, elem);
+}
+
 template <class Op, class Epi>
-int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
+int run_one(Device &d, const Product &g, int splits, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
   CUtensorMap w, t;
   int rc, units;
   if ((rc = operand_maps<Op>(g, err, &w, &t))) return rc;
@@ -348,8 +386,6 @@ int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStr
   p.status = d.status;
   p.timeout_ns = kWaitNs;
   const long long tiles = static_cast<long long>(p.c_tiles) * p.t_tiles;
-  int splits = 1;
-  while (splits < 8 && tiles * splits < 2 * d.num_sms && p.k_blocks >= 4 * splits) splits *= 2;
   // As deep a pipeline as lets the CTAs of one SM share its memory, at least what the split sums need.
   const int per_sm = static_cast<int>(std::min<long long>(4, (tiles * splits + d.num_sms - 1) / d.num_sms));
   const int room = (kSmemPerSm / per_sm - kOneStatic - 2048) / Op::STAGE_BYTES;  // alignment, and 1 KB of the system's
@@ -360,11 +396,24 @@ int run_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStr
   return launched(err);
 }
 
+template <int kElem, bool kWK, bool kTK, class Epi>
+int run_best_one(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
+  using pf::Operands;
+  const Choice c = choose_one(d, g.tokens, g.channels, g.sum, kElem, kTK ? 16 : 128 / kElem);
+  if constexpr (kTK) {
+    if (c.tokens == 16) return run_one<Operands<kElem, kWK, kTK, 16, 1>, Epi>(d, g, c.splits, args, s, err);
+    if (c.tokens == 32) return run_one<Operands<kElem, kWK, kTK, 32, 1>, Epi>(d, g, c.splits, args, s, err);
+  }
+  if (c.tokens == 64) return run_one<Operands<kElem, kWK, kTK, 64, 1>, Epi>(d, g, c.splits, args, s, err);
+  return run_one<Operands<kElem, kWK, kTK, 128, 1>, Epi>(d, g, c.splits, args, s, err);
+}
+
 // Whole waves of 256 x 256 tiles by the pair kernel.  Where the last wave would leave more than half of the pairs idle, its
 // tiles (a rectangle: the last token columns of the raster's last group) go to the one-CTA kernel, which spreads them
 // over the whole GPU: dB of 4096 x 14336 x 8192, 896 tiles on 74 pairs, TAIL.
-template <class Op, class One, class Epi, int kStages>
+template <int kElem, bool kWK, bool kTK, class Epi, int kStages>
 int run_pair(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
+  using Op = pf::Operands<kElem, kWK, kTK, 128, 2>;
   using Cfg = pf::PairConfig<Op, kStages>;
   CUtensorMap w, t;
   int rc, units;
@@ -390,22 +439,15 @@ int run_pair(Device &d, const Product &g, const typename Epi::Args &args, cudaSt
                  args);
   if ((rc = launched(err)) || columns == 0) return rc;
   const int c0 = (p.c_tiles - rows) * 256, t0 = (p.t_tiles - columns) * 256;
-  return run_one<One, Epi>(d, g.part<One>(c0, t0), args.part(c0, t0), s, err);
+  return run_best_one<kElem, kWK, kTK, Epi>(d, g.part<Op>(c0, t0), args.part(c0, t0), s, err);
 }
 
 // Elements, W's and T's order, epilogue -> the kernel for the sizes.
 template <int kElem, bool kWK, bool kTK, class Epi>
 int product(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
-  using pf::Operands;
-  const long long pair_tiles = ((g.channels + 255ll) / 256) * ((g.tokens + 255ll) / 256);
-  if (g.tokens > 128 && pair_tiles >= 32)
-    return run_pair<Operands<kElem, kWK, kTK, 128, 2>, Operands<kElem, kWK, kTK, 128, 1>, Epi, 3>(d, g, args, s, err);
-  if constexpr (kTK) {
-    if (g.tokens <= 16) return run_one<Operands<kElem, kWK, kTK, 16, 1>, Epi>(d, g, args, s, err);
-    if (g.tokens <= 32) return run_one<Operands<kElem, kWK, kTK, 32, 1>, Epi>(d, g, args, s, err);
-  }
-  if (g.tokens <= 64) return run_one<Operands<kElem, kWK, kTK, 64, 1>, Epi>(d, g, args, s, err);
-  return run_one<Operands<kElem, kWK, kTK, 128, 1>, Epi>(d, g, args, s, err);
+  const Choice one = choose_one(d, g.tokens, g.channels, g.sum, kElem, kTK ? 16 : 128 / kElem);
+  if (pair_us(d, g.tokens, g.channels, g.sum, kElem) < one.us) return run_pair<kElem, kWK, kTK, Epi, 3>(d, g, args, s, err);
+  return run_best_one<kElem, kWK, kTK, Epi>(d, g, args, s, err);
 }
 
 }  // namespace
