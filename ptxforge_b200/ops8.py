@@ -18,7 +18,6 @@ allocated on that stream.  Calls do not wait for the GPU: ops8_status() says whe
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 from typing import NamedTuple
@@ -28,7 +27,7 @@ import ptxforge_b200 as _pf
 _F32, _BF16 = 0, 2  # pf_dtype
 _ERR_BYTES = 256
 _local = threading.local()  # each thread's error text
-_here = contextlib.nullcontext()
+_functions = {}  # the library's entry points by name
 torch = None  # imported by the first call: the package loads without it
 _raw_stream = None  # torch's current stream of a device index, as a handle
 
@@ -86,20 +85,30 @@ def _check(x, name, dtype, shape, device):
 
 
 def _on(stream, device):
-    """(the stream's handle, a context in which torch allocates on that stream)."""
+    """(the stream's handle, the stream on which torch is to allocate, None for the current one)."""
     if stream is None:
-        return _raw_stream(device), _here
+        return _raw_stream(device), None
     handle = _pf._stream(stream)
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
-    return handle, torch.cuda.stream(stream)
+    return handle, stream
+
+
+def _empty(on, dtype, device, *size):
+    if on is None:
+        return torch.empty(*size, dtype=dtype, device=device)
+    with torch.cuda.stream(on):
+        return torch.empty(*size, dtype=dtype, device=device)
 
 
 def _call(name: str, *args):
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_pf.load_library(), name)
     err = getattr(_local, "err", None)
     if err is None:
         err = _local.err = ctypes.create_string_buffer(_ERR_BYTES)
-    rc = getattr(_pf.load_library(), name)(*args, err, _ERR_BYTES)
+    rc = fn(*args, err, _ERR_BYTES)
     if rc:
         raise _pf.PFError(rc, f"{name}: {err.value.decode()}")
 
@@ -120,12 +129,11 @@ def quantize_s8(X, axis: int = 1, codes=None, scale=None, *, stream=None):
     rows, cols, ldx = _matrix(X, "X")
     n = _axis(axis, rows, cols)
     dev = X.get_device()
-    handle, here = _on(stream, dev)
-    with here:
-        if codes is None:
-            codes = torch.empty((rows, cols), dtype=torch.int8, device=X.device)
-        if scale is None:
-            scale = torch.empty(n, dtype=torch.float32, device=X.device)
+    handle, on = _on(stream, dev)
+    if codes is None:
+        codes = _empty(on, torch.int8, X.device, rows, cols)
+    if scale is None:
+        scale = _empty(on, torch.float32, X.device, n)
     ldq = _matrix(codes, "codes", torch.int8, (rows, cols), dev)[2]
     _vector(scale, "scale", n, dev)
     _call("pf_quantize_s8", dev, src, rows, cols, X.data_ptr(), ldx, axis, codes.data_ptr(), ldq,
@@ -141,10 +149,9 @@ def dequantize_s8(codes, scale, axis: int = 1, out=None, *, dtype=None, stream=N
     _vector(scale, "scale", _axis(axis, rows, cols), dev)
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
     dst = _type_code(dtype, "dtype")
-    handle, here = _on(stream, dev)
+    handle, on = _on(stream, dev)
     if out is None:
-        with here:
-            out = torch.empty((rows, cols), dtype=dtype, device=codes.device)
+        out = _empty(on, dtype, codes.device, rows, cols)
     ldx = _matrix(out, "out", dtype, (rows, cols), dev)[2]
     _call("pf_dequantize_s8", dev, rows, cols, codes.data_ptr(), ldq, scale.data_ptr(), axis, dst,
           out.data_ptr(), ldx, handle)
@@ -168,16 +175,14 @@ def gemm_s8(A, B, scale_a, scale_b, bias=None, C=None, *, gelu: bool = False, dt
         _vector(bias, "bias", N, dev)
     dtype = dtype or (C.dtype if C is not None else torch.bfloat16)
     out = _type_code(dtype, "dtype")
-    handle, here = _on(stream, dev)
+    handle, on = _on(stream, dev)
     if C is None:
-        with here:
-            C = torch.empty((M, N), dtype=dtype, device=A.device)
+        C = _empty(on, dtype, A.device, M, N)
     ldc = _matrix(C, "C", dtype, (M, N), dev)[2]
     a, b, space = A.data_ptr(), B.data_ptr(), None
     size = _pf.load_library().pf_gemm_s8_workspace(M, N, K, a, lda, b, ldb)  # 0 where rows start on 16-byte boundaries
     if size:
-        with here:
-            space = torch.empty(size, dtype=torch.uint8, device=A.device)  # back to the stream's pool on return
+        space = _empty(on, torch.uint8, A.device, size)  # back to the stream's pool on return
     _call("pf_gemm_s8", dev, M, N, K, a, lda, b, ldb, scale_a.data_ptr(), scale_b.data_ptr(),
           None if bias is None else bias.data_ptr(), int(gelu), out, C.data_ptr(), ldc,
           None if space is None else space.data_ptr(), size, handle)
@@ -211,13 +216,12 @@ def gemm_bias_gelu_checkpoint(A, B, bias, C=None, *, keep_input: bool = True, st
     if K2 != K:
         raise ValueError(f"shape mismatch: A {tuple(A.shape)}, B {tuple(B.shape)}")
     _vector(bias, "bias", N, dev)
-    handle, here = _on(stream, dev)
-    with here:
-        if C is None:
-            C = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
-        grad_codes = torch.empty((M, N), dtype=torch.uint8, device=A.device)
-        a_codes = torch.empty((M, K), dtype=torch.int8, device=A.device) if keep_input else None
-        a_scale = torch.empty(M, dtype=torch.float32, device=A.device) if keep_input else None
+    handle, on = _on(stream, dev)
+    if C is None:
+        C = _empty(on, torch.bfloat16, A.device, M, N)
+    grad_codes = _empty(on, torch.uint8, A.device, M, N)
+    a_codes = _empty(on, torch.int8, A.device, M, K) if keep_input else None
+    a_scale = _empty(on, torch.float32, A.device, M) if keep_input else None
     _matrix(C, "C", torch.bfloat16, (M, N), dev, contiguous=True)
     _call("pf_gemm_bias_gelu_checkpoint", dev, M, N, K, A.data_ptr(), B.data_ptr(), bias.data_ptr(), C.data_ptr(),
           a_codes.data_ptr() if keep_input else None, a_scale.data_ptr() if keep_input else None, grad_codes.data_ptr(),
@@ -244,13 +248,12 @@ def gemm_bias_gelu_backward(dC, B, checkpoint: Checkpoint, *, need=("dA", "dB", 
         _matrix(checkpoint.a_codes, "checkpoint.a_codes", torch.int8, (M, K), dev, contiguous=True)
         _vector(checkpoint.a_scale, "checkpoint.a_scale", M, dev)
         a, s = checkpoint.a_codes.data_ptr(), checkpoint.a_scale.data_ptr()
-    handle, here = _on(stream, dev)
+    handle, on = _on(stream, dev)
     size = _pf.load_library().pf_gemm_bias_gelu_backward_workspace(M, N, K)
-    with here:
-        dA = torch.empty((M, K), dtype=torch.bfloat16, device=dC.device) if "dA" in need else None
-        dB = torch.empty((K, N), dtype=torch.bfloat16, device=dC.device) if "dB" in need else None
-        dbias = torch.empty(N, dtype=torch.float32, device=dC.device) if "dbias" in need else None
-        space = torch.empty(size, dtype=torch.uint8, device=dC.device)  # back to the stream's pool on return
+    dA = _empty(on, torch.bfloat16, dC.device, M, K) if "dA" in need else None
+    dB = _empty(on, torch.bfloat16, dC.device, K, N) if "dB" in need else None
+    dbias = _empty(on, torch.float32, dC.device, N) if "dbias" in need else None
+    space = _empty(on, torch.uint8, dC.device, size)  # back to the stream's pool on return
     _call("pf_gemm_bias_gelu_backward", dev, M, N, K, dC.data_ptr(), B.data_ptr(), a, s,
           checkpoint.grad_codes.data_ptr(), None if dA is None else dA.data_ptr(), None if dB is None else dB.data_ptr(),
           None if dbias is None else dbias.data_ptr(), space.data_ptr(), size, handle)
@@ -266,10 +269,9 @@ def dequantize_gelu_grad(codes, out=None, *, dtype=None, stream=None):
     dev = codes.get_device()
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
     dst = _type_code(dtype, "dtype")
-    handle, here = _on(stream, dev)
+    handle, on = _on(stream, dev)
     if out is None:
-        with here:
-            out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+        out = _empty(on, dtype, codes.device, *codes.shape)
     _check(out, "out", dtype, codes.shape, dev)
     if not out.is_contiguous():
         raise ValueError("out must be contiguous")
