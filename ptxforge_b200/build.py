@@ -13,6 +13,7 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -74,6 +75,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     units = {u: os.path.join(CSRC, u) for u in UNITS}
     deps = {u: sorted(_includes(src)) + [me] for u, src in units.items()}
     if not force and not _stale(LIB, [d for ds in deps.values() for d in ds]):
+        build_torch()
         return LIB
     os.makedirs(OBJ_DIR, exist_ok=True)
     objs = {u: os.path.join(OBJ_DIR, u[:-3] + ".o") for u in UNITS}
@@ -99,7 +101,28 @@ def build(force: bool = False, verbose: bool = False) -> str:
         f.write(log)
     if verbose:
         print(log)
+    build_torch(force)
     return LIB
+
+
+TORCH_SRC = os.path.join(CSRC, "torch_ops8.cpp")
+TORCH_LIB = os.path.join(HERE, "_ops8.so")
+
+
+def build_torch(force: bool = False) -> str | None:
+    """Build _ops8.so, the 8-bit operators' torch side (a Python module over libpf_b200.so), where torch is installed."""
+    try:
+        from torch.utils import cpp_extension
+    except ImportError:
+        return None
+    if force or _stale(TORCH_LIB, sorted(_includes(TORCH_SRC)) + [os.path.abspath(__file__)]):
+        cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+        include = [INCLUDE, *cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", *(a for d in include for a in ("-isystem", d)), TORCH_SRC,
+              "-o", TORCH_LIB + ".tmp", *(a for d in cpp_extension.library_paths() for a in ("-L", d)), "-lc10", "-lc10_cuda",
+              "-ltorch_cpu", "-ltorch", "-ltorch_python", "-L", HERE, "-lpf_b200", "-Wl,-rpath,$ORIGIN"])
+        os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    return TORCH_LIB
 
 
 # The PTXForge source tree the runner plugs into: $PTXFORGE_REFERENCE, else a `reference` directory beside the

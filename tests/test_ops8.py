@@ -118,7 +118,7 @@ def test_backward_workspace():
     (lambda: pf.gemm_s8(torch.zeros(2, 4), torch.zeros(4, 2), torch.zeros(2), torch.zeros(2)), "int8"),
     (lambda: pf.gemm_s8(torch.zeros(2, 4, dtype=torch.int8), torch.zeros(4, 2), torch.zeros(2), torch.zeros(2)), "CUDA tensor"),
     (lambda: pf.gemm_bias_gelu_checkpoint(torch.zeros(8, 8), torch.zeros(8, 8), torch.zeros(8)), "bfloat16"),
-    (lambda: pf.gemm_bias_gelu_backward(torch.zeros(8, 8), torch.zeros(8, 8), pf.Checkpoint(None, None, None)), "bfloat16"),
+    (lambda: pf.gemm_bias_gelu_backward(torch.zeros(8, 8), torch.zeros(8, 8), pf.Checkpoint(None, None, torch.zeros(8, 8))), "bfloat16"),
     (lambda: pf.gemm_bias_gelu_backward(torch.zeros(8, 8), None, None, need=("dA", "dW")), "dW"),
     (lambda: pf.dequantize_gelu_grad(torch.zeros(8)), "uint8"),
     (lambda: pf.dequantize_gelu_grad(torch.zeros(8, dtype=torch.uint8)), "CUDA tensor"),
