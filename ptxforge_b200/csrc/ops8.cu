@@ -159,7 +159,8 @@ template <class T, int kVec>
 void quantize_rows(const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale, cudaStream_t s) {
   // Many rows: a warp each where its registers hold the row, else a block each, eight vectors a thread -- much in flight
   // and few threads to join.  Few rows: as many threads a row as it can use, so that a lone one is spread over an SM.
-  // Measured, bf16, us: 16384 x 4096 with 2 vectors a thread 52, with 8 HELD8; one row of 4096 HELD1.
+  // Measured, us: 16384 x 4096 bf16 with 2 vectors a thread 52, with 8 43; 65536 x 512 fp32 with 2 and a block a row 69,
+  // with 4 and a warp a row 26.
   const int vecs = (cols + kVec - 1) / kVec;
   const auto launch = [&](auto kernel, dim3 block) {
     pf::launch_pdl(kernel, dim3(blocks_of(rows, block.y)), block, 0, s, x, ldx, rows, cols, q, ldq, scale);
@@ -264,9 +265,13 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // The parts of the backward pass's workspace, in order, each 256-byte aligned.
 struct BackwardSpace {
   size_t dz, a, partial, total;
-  int parts;
+  int col_blocks, rows, parts;
   BackwardSpace(int M, int N, int K) {
-    parts = (M + pf::kDzRows - 1) / pf::kDzRows;
+    // 128 rows a block of the elementwise kernel (and a part of dbias' sums); 32 where that makes too few blocks to keep
+    // the memory busy (1999 x 2048: 6.8 us with 128, 5.3 with 32).
+    col_blocks = (N + pf::kDzCols - 1) / pf::kDzCols;
+    rows = (M + 127) / 128 * static_cast<long long>(col_blocks) < 1024 ? 32 : 128;
+    parts = (M + rows - 1) / rows;
     dz = 0;
     a = dz + round256(size_t(M) * N * sizeof(bf16));
     partial = a + round256(size_t(M) * K * sizeof(bf16));
@@ -291,12 +296,6 @@ struct ProductSpace {
     total = b + (copy_b ? round256(size_t(K) * ldb) : 0);
   }
 };
-
-const void *aligned_copy(const signed char *X, long long ld, int rows, int cols, char *to, long long ld_to, cudaStream_t s) {
-  pf::launch_pdl(&pf::align_rows, dim3(rows), 256, 0, s, reinterpret_cast<const uint8_t *>(X), ld, cols,
-                 reinterpret_cast<uint4 *>(to), ld_to / 16);
-  return to;
-}
 
 // One product: out[t][c] = sum_r T(t, r) W(r, c).  A K-major operand is [t][r] or [c][r], an MN-major one [r][t] or
 // [r][c], with row strides ldt, ldw in elements.
@@ -410,7 +409,8 @@ int run_best_one(Device &d, const Product &g, const typename Epi::Args &args, cu
 
 // Whole waves of 256 x 256 tiles by the pair kernel.  Where the last wave would leave more than half of the pairs idle, its
 // tiles (a rectangle: the last token columns of the raster's last group) go to the one-CTA kernel, which spreads them
-// over the whole GPU: dB of 4096 x 14336 x 8192, 896 tiles on 74 pairs, TAIL.
+// over the whole GPU: dB of 4096 x 14336 from 8192 tokens, 896 tiles on 74
+// pairs: 826 us in whole waves, 651 so.
 template <int kElem, bool kWK, bool kTK, class Epi, int kStages>
 int run_pair(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
   using Op = pf::Operands<kElem, kWK, kTK, 128, 2>;
@@ -527,8 +527,15 @@ int pf_gemm_s8(int device, int M, int N, int K, const signed char *A, long long 
   if ((rc = stream_of(device, stream, err, &s))) return rc;
   Product p{M, N, K, A, B, lda, ldb};
   char *base = static_cast<char *>(workspace);
-  if (w.copy_a) p.T = aligned_copy(A, lda, M, K, base, w.lda, s);
-  if (w.copy_b) p.W = aligned_copy(B, ldb, K, N, base + w.b, w.ldb, s);
+  if (w.total) {
+    if (static_cast<long long>(M) + K > 0x7FFFFFFF) return err(PF_EINVAL, "more than 2^31 rows to align");
+    const pf::AlignRows a{reinterpret_cast<const uint8_t *>(A), lda, K, reinterpret_cast<uint4 *>(base), w.lda / 16};
+    const pf::AlignRows b{reinterpret_cast<const uint8_t *>(B), ldb, N, reinterpret_cast<uint4 *>(base + w.b), w.ldb / 16};
+    const int rows_a = w.copy_a ? M : 0;
+    pf::launch_pdl(&pf::align_rows, dim3(rows_a + (w.copy_b ? K : 0)), 128, 0, s, a, b, rows_a);
+    if (w.copy_a) p.T = base;
+    if (w.copy_b) p.W = base + w.b;
+  }
   p.ldt = w.lda;
   p.ldw = w.ldb;
   if (out == PF_F32)
@@ -595,12 +602,11 @@ int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, 
   char *base = static_cast<char *>(workspace);
   bf16 *dz = reinterpret_cast<bf16 *>(base + w.dz), *a = reinterpret_cast<bf16 *>(base + w.a);
   float *partial = reinterpret_cast<float *>(base + w.partial);
-  const int col_blocks = (N + pf::kDzCols - 1) / pf::kDzCols;
-  const long long dz_blocks = static_cast<long long>(col_blocks) * w.parts, blocks = dz_blocks + (dB ? M : 0);
+  const long long dz_blocks = static_cast<long long>(w.col_blocks) * w.parts, blocks = dz_blocks + (dB ? M : 0);
   if (blocks > 0x7FFFFFFF) return err(PF_EINVAL, "more than 2^31 blocks");
   float *sums = dbias && w.parts == 1 ? dbias : partial;
   pf::launch_pdl(&pf::backward_operands, dim3(static_cast<unsigned>(blocks)), 256, 0, s, static_cast<const bf16 *>(dC), grad_codes,
-                 dB ? a_scale : static_cast<const float *>(nullptr), M, N, static_cast<int>(dz_blocks), col_blocks, dz, sums,
+                 dB ? a_scale : static_cast<const float *>(nullptr), M, N, static_cast<int>(dz_blocks), w.col_blocks, w.rows, dz, sums,
                  reinterpret_cast<const int8_t *>(a_codes), K, a);
   if (dbias && w.parts > 1)
     pf::launch_pdl(&pf::sum_row_blocks, dim3(blocks_of(N, 32)), 256, 0, s, static_cast<const float *>(partial), w.parts, N, dbias);

@@ -506,10 +506,23 @@ __global__ void __launch_bounds__(256) dequantize_grad(const uint8_t *D, long lo
 // Rows of bytes that start anywhere -> rows of whole 16-byte words.  Each word is put together from the aligned
 // 4-byte words that hold its bytes; a word with no byte of the row is not read.  What follows a row's end is whatever
 // shares its last word, and is never used.
-__global__ void align_rows(const uint8_t *X, long long ld, int cols, uint4 *Y, long long ld_y) {
+// One launch for two matrices: a block a row, the first rows_a of them of `a`.
+struct AlignRows {
+  const uint8_t *X;
+  long long ld;
+  int cols;
+  uint4 *Y;
+  long long ld_y;
+};
+__global__ void __launch_bounds__(128) align_rows(const AlignRows a, const AlignRows b, int rows_a) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const long long r = blockIdx.x;
+  const bool second = static_cast<int>(blockIdx.x) >= rows_a;
+  const uint8_t *X = second ? b.X : a.X;
+  uint4 *Y = second ? b.Y : a.Y;
+  const long long ld = second ? b.ld : a.ld, ld_y = second ? b.ld_y : a.ld_y;
+  const long long r = static_cast<int>(blockIdx.x) - (second ? rows_a : 0);
+  const int cols = second ? b.cols : a.cols;
   const uintptr_t row = reinterpret_cast<uintptr_t>(X + r * ld);
   const unsigned shift = 8 * static_cast<unsigned>(row & 3);
   const uint32_t *x = reinterpret_cast<const uint32_t *>(row & ~uintptr_t(3));
@@ -526,13 +539,14 @@ __global__ void align_rows(const uint8_t *X, long long ld, int cols, uint4 *Y, l
 // ------------------------------------------------------------------------------------------------
 // the backward pass's elementwise part
 // ------------------------------------------------------------------------------------------------
-// Blocks below dz_blocks: m dz = m dC d~ (rounded once to bf16) of 256 columns x kDzRows rows and, from the unrounded dz,
+// Blocks below dz_blocks: m dz = m dC d~ (rounded once to bf16) of 256 columns x dz_rows rows and, from the unrounded dz,
 // their column sums in fp32 (`sums` [row block][column]; with one row block that is dbias).  dC k is exact in fp32 (8 by
 // 8 bits), so dz is rounded once by 1 / 200.  The blocks after them: the input's q 2^e in bf16, exact, a row each.
 // a_scale may be null (m = 1, no input wanted).
-constexpr int kDzRows = 128, kDzCols = 256;
+constexpr int kDzCols = 256;
 __global__ void __launch_bounds__(256) backward_operands(const __nv_bfloat16 *dC, const uint8_t *D, const float *a_scale,
-                                                         int M, int N, int dz_blocks, int col_blocks, __nv_bfloat16 *dz,
+                                                         int M, int N, int dz_blocks, int col_blocks, int dz_rows,
+                                                         __nv_bfloat16 *dz,
                                                          float *sums, const int8_t *Q, int K, __nv_bfloat16 *input) {
   __shared__ float sh[8][kDzCols];
   grid_launch_dependents();
@@ -547,7 +561,7 @@ __global__ void __launch_bounds__(256) backward_operands(const __nv_bfloat16 *dC
   const int c = (blockIdx.x - rb * col_blocks) * kDzCols + lane * 8;
   float sum[8] = {};
   if (c < N) {
-    const int r0 = rb * kDzRows + row, r1 = min(M, (rb + 1) * kDzRows);
+    const int r0 = rb * dz_rows + row, r1 = min(M, (rb + 1) * dz_rows);
 #pragma unroll 4
     for (int r = r0; r < r1; r += 8) {
       const long long i = static_cast<long long>(r) * N + c;
