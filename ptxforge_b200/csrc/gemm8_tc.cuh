@@ -509,7 +509,8 @@ __global__ void __launch_bounds__(kOneThreads, 4)
       else join_sums<TOKENS, 8, Epi>(args, c0, p.channels, base, rank, warp - 2, lane, t0, tokens, sc);
     }
     __syncwarp();
-    cluster_sync();  // nobody leaves while its shared memory may be read
+    cluster_arrive_relaxed();
+    cluster_wait();  // nobody leaves while its shared memory may be read
   } else {
     __syncthreads();
   }
@@ -729,7 +730,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
       }
     }
   }
-  // Neither CTA releases TMEM or exits while its peer may still address it.
+  // Neither CTA releases TMEM or exits while its peer may still address it (with a release: the last remote arrivals
+  // on `tempty` land before the leader may leave).
   __syncwarp();
   cluster_sync();
   if (warp == 1) {

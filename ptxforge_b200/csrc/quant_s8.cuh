@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(256, 3) quantize_strips_s8(const __grid_consta
     if (rank == 0 && c0 + static_cast<int>(threadIdx.x) < cols) scale[c0 + threadIdx.x] = s;
   }
   __syncthreads();
+  cluster_arrive_relaxed();  // the others' maxima were read
   if (c < cols) {  // whole vectors: cols is a multiple of kVec
     float s[kVec], inv[kVec];
     bool bad = false;
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(256, 3) quantize_strips_s8(const __grid_consta
     }
   }
   __syncwarp();
-  cluster_sync();  // nobody leaves while its maxima may be read
+  cluster_wait();  // nobody leaves while its maxima may be read
 }
 
 // Any matrix, two passes: 32 vectors of columns x kColRows rows a block.  First the largest abs_bits of each column into
