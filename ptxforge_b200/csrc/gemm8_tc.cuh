@@ -534,44 +534,72 @@ __device__ __forceinline__ void pair_tile(int i, const Gemm8Params &p, int &ct, 
   tt = r / rows;
 }
 
-template <class Op, int kStages>
+// A pair kernel walks the tiles of one product, or of two, one after the other: dA and dB of a layer keep the pairs busy
+// together where either alone would leave a wave unfilled, and share the launch.
+template <class Op, class Epi>
+struct Job {
+  typedef Op Operands;
+  typedef Epi Epilogue;
+  typedef typename Epi::Args Args;
+  static constexpr bool kNone = false;
+};
+struct NoJob {
+  struct Args {};
+  static constexpr bool kNone = true;
+};
+
+template <class J, int kStages>
 struct PairConfig {
+  typedef typename J::Operands Op;
   static constexpr int STAGES = kStages;
   static constexpr int EPI_WARPS = 8;    // two to a quarter of the TMEM lanes, each with half of the tokens
   static constexpr int EPI_BLOCKS = 4;   // blocks of 32 tokens a warp
   static constexpr int THREADS = 64 + EPI_WARPS * 32;
   static constexpr int NUM_BARS = 2 * STAGES + 4 + 1;
   static constexpr int SMEM_BYTES = 1024 + STAGES * Op::STAGE_BYTES + NUM_BARS * 8 + 16;
-  static constexpr uint32_t IDESC = Op::idesc(256, 256);
   static_assert(Op::TOKENS == 128, "each CTA of a pair supplies 128 tokens");
   static_assert(SMEM_BYTES <= 232448, "shared memory per block exceeds the sm_100 opt-in limit");
 };
 
-template <class Op, class Epi, int kStages>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStages>::THREADS, 1)
-    gemm8_pair(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const Gemm8Params p,
-               const typename Epi::Args args) {
-  using Cfg = PairConfig<Op, kStages>;
+template <int kStages, class J1, class J2>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<J1, kStages>::THREADS, 1)
+    gemm8_pair(const __grid_constant__ CUtensorMap tmW1, const __grid_constant__ CUtensorMap tmT1,
+               const __grid_constant__ CUtensorMap tmW2, const __grid_constant__ CUtensorMap tmT2, const Gemm8Params p1,
+               const Gemm8Params p2, const typename J1::Args args1, const typename J2::Args args2) {
+  using Cfg = PairConfig<J1, kStages>;
+  constexpr int W_BYTES = Cfg::Op::W_BYTES, T_BYTES = Cfg::Op::T_BYTES, STAGE_BYTES = Cfg::Op::STAGE_BYTES;
   __shared__ __align__(16) float scalars[Cfg::EPI_WARPS][Cfg::EPI_BLOCKS * 32];
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t *sW = smem, *sT = smem + Cfg::STAGES * Op::W_BYTES;
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Cfg::STAGES * Op::STAGE_BYTES);  // leader: both CTAs' bytes landed
-  uint64_t *empty = full + Cfg::STAGES;                                                 // both: the stage was read
-  uint64_t *tfull = empty + Cfg::STAGES;                                                // both: accumulator ready
-  uint64_t *tempty = tfull + 2;                                                         // leader: accumulator drained
-  uint64_t *drain = tempty + 2;                                                         // leader: all MMAs complete
+  uint8_t *sW = smem, *sT = smem + Cfg::STAGES * W_BYTES;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Cfg::STAGES * STAGE_BYTES);  // leader: both CTAs' bytes landed
+  uint64_t *empty = full + Cfg::STAGES;                                             // both: the stage was read
+  uint64_t *tfull = empty + Cfg::STAGES;                                            // both: accumulator ready
+  uint64_t *tempty = tfull + 2;                                                     // leader: accumulator drained
+  uint64_t *drain = tempty + 2;                                                     // leader: all MMAs complete
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(drain + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int tiles = p.tiles;
+  const int tiles = p1.tiles + (J2::kNone ? 0 : p2.tiles);
+  // f(job, W's map, T's map, parameters, epilogue arguments, the job's tile) for tile i of the launch
+  auto with_tile = [&](int i, auto f) {
+    if constexpr (!J2::kNone) {
+      static_assert(J2::Operands::W_BYTES == W_BYTES && J2::Operands::T_BYTES == T_BYTES, "the jobs share the stages");
+      if (i >= p1.tiles) return f(J2{}, &tmW2, &tmT2, p2, args2, i - p1.tiles);
+    }
+    return f(J1{}, &tmW1, &tmT1, p1, args1, i);
+  };
 
   if (threadIdx.x == 0) {
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmT);
+    tma_prefetch_desc(&tmW1);
+    tma_prefetch_desc(&tmT1);
+    if (!J2::kNone) {
+      tma_prefetch_desc(&tmW2);
+      tma_prefetch_desc(&tmT2);
+    }
     for (int s = 0; s < Cfg::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -594,7 +622,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   auto fail = [&](unsigned bit) {
-    atomicOr(p.status, bit);
+    atomicOr(p1.status, bit);
     *abort_flag = 1;
   };
 
@@ -603,25 +631,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
       int stage = 0;
       uint32_t phase = 0;
       int issued = 0;
-      bool ok = true;
-      for (int i = pair; ok && i < tiles; i += pairs) {
+      auto produce = [&](auto job, const CUtensorMap *tmW, const CUtensorMap *tmT, const Gemm8Params &p, const auto &, int i) {
+        using Op = typename decltype(job)::Operands;
         int ct, tt;
         pair_tile(i, p, ct, tt);
         const int c0 = ct * 256 + static_cast<int>(rank) * 128, t0 = tt * 256 + static_cast<int>(rank) * 128;
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, p.timeout_ns, abort_flag)) {
             fail(kErrProducerWait);
-            ok = false;
-            break;
+            return false;
           }
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * Op::STAGE_BYTES);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * STAGE_BYTES);
           if (issued == 0) grid_dependency_wait();
           const uint32_t bar = pair_leader_addr(smem_u32(&full[stage]));
-          Op::template load<Op::W_K, 128>(sW + stage * Op::W_BYTES, c0, kb, [&](uint8_t *dst, int x, int y) {
-            tma_load_2d_pair(dst, &tmW, bar, x, y);
+          Op::template load<Op::W_K, 128>(sW + stage * W_BYTES, c0, kb, [&](uint8_t *dst, int x, int y) {
+            tma_load_2d_pair(dst, tmW, bar, x, y);
           });
-          Op::template load<Op::T_K, 128>(sT + stage * Op::T_BYTES, t0, kb, [&](uint8_t *dst, int x, int y) {
-            tma_load_2d_pair(dst, &tmT, bar, x, y);
+          Op::template load<Op::T_K, 128>(sT + stage * T_BYTES, t0, kb, [&](uint8_t *dst, int x, int y) {
+            tma_load_2d_pair(dst, tmT, bar, x, y);
           });
           ++issued;
           if (++stage == Cfg::STAGES) {
@@ -629,13 +656,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
             phase ^= 1u;
           }
         }
-      }
+        return true;
+      };
+      bool ok = true;
+      for (int i = pair; ok && i < tiles; i += pairs) ok = with_tile(i, produce);
       if (!ok && rank == 0) {
         // Loads in flight land before the pair may exit (bounded).
         for (int s = 0; s < Cfg::STAGES && s < issued; ++s) {
           const uint32_t ph = (s < stage) ? phase : (phase ^ 1u);
           volatile int no_abort = 0;
-          if (!mbar_wait(&full[s], ph, p.timeout_ns, &no_abort)) atomicOr(p.status, kErrTeardownWait);
+          if (!mbar_wait(&full[s], ph, p1.timeout_ns, &no_abort)) atomicOr(p1.status, kErrTeardownWait);
         }
       }
     }
@@ -646,29 +676,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
-      bool ok = true;
-      for (int i = pair; ok && i < tiles; i += pairs) {
+      auto multiply = [&](auto job, const CUtensorMap *, const CUtensorMap *, const Gemm8Params &p, const auto &, int) {
+        using Op = typename decltype(job)::Operands;
+        constexpr uint32_t IDESC = Op::idesc(256, 256);
         if (!mbar_wait_cluster(&tempty[acc], acc_phase ^ 1u, p.timeout_ns, abort_flag)) {
           fail(kErrMmaWait);
-          ok = false;
-          break;
+          return false;
         }
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(acc * 256);
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!mbar_wait(&full[stage], phase, p.timeout_ns, abort_flag)) {
             fail(kErrMmaWait);
-            ok = false;
-            break;
+            return false;
           }
           tc_fence_after();
-          const uint32_t w = smem_u32(sW + stage * Op::W_BYTES), t = smem_u32(sT + stage * Op::T_BYTES);
+          const uint32_t w = smem_u32(sW + stage * W_BYTES), t = smem_u32(sT + stage * T_BYTES);
 #pragma unroll
           for (int k = 0; k < Op::STEPS; ++k) {
             const uint64_t wd = Op::template desc<Op::W_K, 128>(w, k), td = Op::template desc<Op::T_K, 128>(t, k);
             const uint32_t accumulate = (kb != 0 || k != 0) ? 1u : 0u;
-            if constexpr (Op::ELEM == 2) tc_mma_f16_pair(d, wd, td, Cfg::IDESC, accumulate);
-            else tc_mma_i8_pair(d, wd, td, Cfg::IDESC, accumulate);
+            if constexpr (Op::ELEM == 2) tc_mma_f16_pair(d, wd, td, IDESC, accumulate);
+            else tc_mma_i8_pair(d, wd, td, IDESC, accumulate);
           }
           tc_commit_pair_mc(&empty[stage], 0x3);
           if (++stage == Cfg::STAGES) {
@@ -676,16 +705,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
             phase ^= 1u;
           }
         }
-        if (!ok) break;
         tc_commit_pair_mc(&tfull[acc], 0x3);
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1u;
         }
-      }
+        return true;
+      };
+      for (int i = pair; i < tiles; i += pairs)
+        if (!with_tile(i, multiply)) break;
       tc_commit_pair(drain);
       volatile int no_abort = 0;
-      if (!mbar_wait(drain, 0, p.timeout_ns, &no_abort)) atomicOr(p.status, kErrTeardownWait);
+      if (!mbar_wait(drain, 0, p1.timeout_ns, &no_abort)) atomicOr(p1.status, kErrTeardownWait);
     }
     grid_launch_dependents();
   } else {
@@ -695,7 +726,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
     float *mine = scalars[warp - 2];
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int i = pair; i < tiles; i += pairs) {
+    auto finish = [&](auto job, const CUtensorMap *, const CUtensorMap *, const Gemm8Params &p, const auto &args, int i) {
+      using Epi = typename decltype(job)::Epilogue;
       int ct, tt;
       pair_tile(i, p, ct, tt);
       const int t0 = tt * 256 + half * 128;
@@ -705,7 +737,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
       const bool waited = mbar_wait(&tfull[acc], acc_phase, p.timeout_ns, abort_flag);
       if (!__all_sync(0xffffffffu, waited)) {
         if (lane == 0) fail(kErrEpilogueWait);
-        break;
+        return false;
       }
       tc_fence_after();
       const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256 + half * 128);
@@ -728,7 +760,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<Op, kStag
         acc = 0;
         acc_phase ^= 1u;
       }
-    }
+      return true;
+    };
+    for (int i = pair; i < tiles; i += pairs)
+      if (!with_tile(i, finish)) break;
   }
   // Neither CTA releases TMEM or exits while its peer may still address it (with a release: the last remote arrivals
   // on `tempty` land before the leader may leave).

@@ -11,6 +11,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
+#include <type_traits>
 
 #include "pf_b200.h"
 #include "gemm8_tc.cuh"
@@ -362,12 +363,20 @@ Choice choose_one(const Device &d, int tokens, int channels, int sum, int elem, 
   }
   return best;
 }
-double pair_us(const Device &d, int tokens, int channels, int sum, int elem) {
-  const double tiles = std::ceil(channels / 256.0) * std::ceil(tokens / 256.0), waves = tiles / (d.num_sms / 2);
+// n1 tiles of k1 k-blocks, then n2 of k2, dealt to the pairs in turn: the pair with the most.
+double pair_us(const Device &d, long long n1, int k1, long long n2, int k2) {
+  const long long pairs = d.num_sms / 2, over = (n1 + n2) % pairs;
+  double most = 0;
   // a short last wave goes to the one-CTA kernel (run_pair): about half a wave and a launch
-  const double part = waves - std::floor(waves), whole = waves > 1 && part > 0 && part <= 0.5 ? std::floor(waves) + 0.5 : std::ceil(waves);
-  return 11.5 + 0.28 * whole * k_blocks_of(sum, elem);
+  const bool cut = n1 + n2 > pairs && 2 * over <= pairs && over <= n2;
+  const long long n = n1 + n2 - (cut ? over : 0);
+  for (long long p = 0; p < pairs; ++p) {
+    const long long all = n > p ? (n - 1 - p) / pairs + 1 : 0, one = n1 > p ? (n1 - 1 - p) / pairs + 1 : 0;
+    most = std::max(most, double(one) * k1 + double(all - one) * k2);
+  }
+  return 11.5 + 0.28 * (most + (cut && over ? 0.5 * k2 : 0.0));
 }
+long long pair_tiles(const Product &g) { return (g.channels + 255ll) / 256 * ((g.tokens + 255ll) / 256); }
 
 template <class Op, class Epi>
 int run_one(Device &d, const Product &g, int splits, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
@@ -407,48 +416,103 @@ int run_best_one(Device &d, const Product &g, const typename Epi::Args &args, cu
   return run_one<Operands<kElem, kWK, kTK, 128, 1>, Epi>(d, g, c.splits, args, s, err);
 }
 
+// One product's part of a pair launch.
+template <int kElem, bool kWK, bool kTK, class Epi_>
+struct PairJob {
+  static constexpr int ELEM = kElem;
+  static constexpr bool WK = kWK, TK = kTK;
+  typedef Epi_ Epi;
+  typedef pf::Operands<kElem, kWK, kTK, 128, 2> Op;
+  typedef pf::Job<Op, Epi> Kernel;
+  Product g;
+  typename Epi::Args args;
+  CUtensorMap w, t;
+  pf::Gemm8Params p = {};
+  int prepare(Device &d, const Err &err) {
+    int rc;
+    if ((rc = operand_maps<Op>(g, err, &w, &t))) return rc;
+    p.channels = g.channels;
+    p.tokens = g.tokens;
+    p.c_tiles = (g.channels + 255) / 256;
+    p.t_tiles = (g.tokens + 255) / 256;
+    p.k_blocks = (g.sum + Op::BK - 1) / Op::BK;
+    p.group = std::min(16, p.c_tiles);
+    p.status = d.status;
+    p.timeout_ns = kWaitNs;
+    const long long tiles = static_cast<long long>(p.c_tiles) * p.t_tiles;
+    if (tiles > (1ll << 29)) return err(PF_EINVAL, "more than 2^29 tiles of 256 x 256");
+    p.tiles = static_cast<int>(tiles);
+    return PF_OK;
+  }
+};
+
 // Whole waves of 256 x 256 tiles by the pair kernel.  Where the last wave would leave more than half of the pairs idle, its
 // tiles (a rectangle: the last token columns of the raster's last group) go to the one-CTA kernel, which spreads them
-// over the whole GPU: dB of 4096 x 14336 from 8192 tokens, 896 tiles on 74
-// pairs: 826 us in whole waves, 651 so.
-template <int kElem, bool kWK, bool kTK, class Epi, int kStages>
-int run_pair(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
-  using Op = pf::Operands<kElem, kWK, kTK, 128, 2>;
-  using Cfg = pf::PairConfig<Op, kStages>;
-  CUtensorMap w, t;
+// over the whole GPU: dB of 4096 x 14336 from 8192 tokens, 896 tiles on 74 pairs: 826 us in whole waves, 651 so.
+// `first`: a product whose tiles come before `last`'s, or null.
+template <class First, class Last>
+int run_pair(Device &d, First *first, Last &last, cudaStream_t s, const Err &err) {
+  constexpr int kStages = 3;
+  typedef typename Last::Kernel J;
+  using Cfg = pf::PairConfig<J, kStages>;
+  constexpr bool kTwo = !std::is_same<First, Last>::value;
   int rc, units;
-  if ((rc = operand_maps<Op>(g, err, &w, &t))) return rc;
-  const void *func = reinterpret_cast<const void *>(&pf::gemm8_pair<Op, Epi, kStages>);
+  if ((rc = last.prepare(d, err))) return rc;
+  int before = 0;
+  if constexpr (kTwo) {
+    if ((rc = first->prepare(d, err))) return rc;
+    before = first->p.tiles;
+  }
+  const void *func;
+  if constexpr (kTwo) func = reinterpret_cast<const void *>(&pf::gemm8_pair<kStages, typename First::Kernel, J>);
+  else func = reinterpret_cast<const void *>(&pf::gemm8_pair<kStages, J, pf::NoJob>);
   if ((rc = kernel_units(d, func, Cfg::SMEM_BYTES, Cfg::THREADS, err, &units))) return rc;
-  pf::Gemm8Params p = {};
-  p.channels = g.channels;
-  p.tokens = g.tokens;
-  p.c_tiles = (g.channels + 255) / 256;
-  p.t_tiles = (g.tokens + 255) / 256;
-  p.k_blocks = (g.sum + Op::BK - 1) / Op::BK;
-  p.group = std::min(16, p.c_tiles);
-  p.status = d.status;
-  p.timeout_ns = kWaitNs;
-  const long long tiles = static_cast<long long>(p.c_tiles) * p.t_tiles;
-  if (tiles > (1ll << 30)) return err(PF_EINVAL, "more than 2^30 tiles of 256 x 256");
-  const int last = static_cast<int>(tiles % units), rows = p.c_tiles - (p.c_tiles - 1) / p.group * p.group;
-  int columns = (last + rows - 1) / rows;
+  pf::Gemm8Params &p = last.p;
+  const int tiles = before + p.tiles, over = tiles % units, rows = p.c_tiles - (p.c_tiles - 1) / p.group * p.group;
+  int columns = (over + rows - 1) / rows;
   if (tiles < units || 2 * columns * rows > units || columns >= p.t_tiles) columns = 0;
-  p.tiles = static_cast<int>(tiles) - columns * rows;
-  pf::launch_pdl(&pf::gemm8_pair<Op, Epi, kStages>, dim3(2 * std::min(p.tiles, units)), Cfg::THREADS, Cfg::SMEM_BYTES, s, w, t, p,
-                 args);
+  p.tiles -= columns * rows;
+  const dim3 grid(2 * std::min(tiles - columns * rows, units));
+  if constexpr (kTwo)
+    pf::launch_pdl(&pf::gemm8_pair<kStages, typename First::Kernel, J>, grid, Cfg::THREADS, Cfg::SMEM_BYTES, s, first->w, first->t,
+                   last.w, last.t, first->p, p, first->args, last.args);
+  else
+    pf::launch_pdl(&pf::gemm8_pair<kStages, J, pf::NoJob>, grid, Cfg::THREADS, Cfg::SMEM_BYTES, s, last.w, last.t, last.w, last.t, p, p,
+                   last.args, pf::NoJob::Args{});
   if ((rc = launched(err)) || columns == 0) return rc;
   const int c0 = (p.c_tiles - rows) * 256, t0 = (p.t_tiles - columns) * 256;
-  return run_best_one<kElem, kWK, kTK, Epi>(d, g.part<Op>(c0, t0), args.part(c0, t0), s, err);
+  return run_best_one<Last::ELEM, Last::WK, Last::TK, typename Last::Epi>(d, last.g.template part<typename Last::Op>(c0, t0),
+                                                                          last.args.part(c0, t0), s, err);
 }
 
 // Elements, W's and T's order, epilogue -> the kernel for the sizes.
 template <int kElem, bool kWK, bool kTK, class Epi>
 int product(Device &d, const Product &g, const typename Epi::Args &args, cudaStream_t s, const Err &err) {
   const Choice one = choose_one(d, g.tokens, g.channels, g.sum, kElem, kTK ? 16 : 128 / kElem);
-  if (pair_us(d, g.tokens, g.channels, g.sum, kElem) < one.us) return run_pair<kElem, kWK, kTK, Epi, 3>(d, g, args, s, err);
+  if (pair_us(d, 0, 0, pair_tiles(g), k_blocks_of(g.sum, kElem)) < one.us) {
+    PairJob<kElem, kWK, kTK, Epi> job{g, args};
+    return run_pair(d, &job, job, s, err);
+  }
   return run_best_one<kElem, kWK, kTK, Epi>(d, g, args, s, err);
 }
+
+// dA and dB: one pair launch over both where that is estimated to be shorter than each by its own best kernel.
+template <class EpiA, class EpiB>
+int two_products(Device &d, const Product &ga, const typename EpiA::Args &aa, const Product &gb, const typename EpiB::Args &ab,
+                 cudaStream_t s, const Err &err) {
+  const auto alone = [&](const Product &g, int least) {
+    return std::min(choose_one(d, g.tokens, g.channels, g.sum, 2, least).us, pair_us(d, 0, 0, pair_tiles(g), k_blocks_of(g.sum, 2)));
+  };
+  const double both = pair_us(d, pair_tiles(ga), k_blocks_of(ga.sum, 2), pair_tiles(gb), k_blocks_of(gb.sum, 2));
+  if (both < alone(ga, 16) + alone(gb, 64)) {
+    PairJob<2, true, true, EpiA> a{ga, aa};
+    PairJob<2, false, false, EpiB> b{gb, ab};
+    return run_pair(d, &a, b, s, err);
+  }
+  const int rc = product<2, true, true, EpiA>(d, ga, aa, s, err);
+  return rc ? rc : product<2, false, false, EpiB>(d, gb, ab, s, err);
+}
+
 
 }  // namespace
 
@@ -610,18 +674,13 @@ int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, 
                  reinterpret_cast<const int8_t *>(a_codes), K, a);
   if (dbias && w.parts > 1)
     pf::launch_pdl(&pf::sum_row_blocks, dim3(blocks_of(N, 32)), 256, 0, s, static_cast<const float *>(partial), w.parts, N, dbias);
-  if (dA) {
-    const Product g{M, K, N, dz, B, N, N};
-    bf16 *out = static_cast<bf16 *>(dA);
-    rc = dB ? product<2, true, true, pf::EpilogueBf16<true>>(*d, g, {a_scale, out, K}, s, err)
-            : product<2, true, true, pf::EpilogueBf16<false>>(*d, g, {nullptr, out, K}, s, err);
-    if (rc) return rc;
-  }
-  if (dB) {
-    if ((rc = product<2, false, false, pf::EpilogueBf16<false>>(*d, Product{K, N, M, a, dz, K, N},
-                                                         {nullptr, static_cast<bf16 *>(dB), N}, s, err)))
-      return rc;
-  }
+  typedef pf::EpilogueBf16<true> Divided;
+  typedef pf::EpilogueBf16<false> Plain;
+  const Product ga{M, K, N, dz, B, N, N}, gb{K, N, M, a, dz, K, N};
+  bf16 *out_a = static_cast<bf16 *>(dA), *out_b = static_cast<bf16 *>(dB);
+  if (dA && dB) return two_products<Divided, Plain>(*d, ga, {a_scale, out_a, K}, gb, {nullptr, out_b, N}, s, err);
+  if (dA) return product<2, true, true, Plain>(*d, ga, {nullptr, out_a, K}, s, err);
+  if (dB) return product<2, false, false, Plain>(*d, gb, {nullptr, out_b, N}, s, err);
   return launched(err);
 }
 
