@@ -262,7 +262,8 @@ int pf_gemm_bias_gelu_noalloc(int device, pf_dtype dtype, const pf_tile *tile, i
  *     device before that) and made from several threads.  Calls that overlap on the GPU need workspaces of
  *     their own, and so do two captured graphs that may.
  *   - Matrices are row-major; ld* are row strides in elements, at least the row's length.
- *   - rows, M = 0 (no tokens) is a call that writes nothing, or the zero sums that are over tokens.
+ *   - Sizes are at most 2^30.  rows, M = 0 (no tokens) is a call that writes nothing, or the sums and scales that are
+ *     over tokens: zeros, and the least scale.
  *   - `err` (may be NULL) receives a message of at most `err_len` bytes on failure.
  *   - Kernel-side waits are bounded by 4 s; one that ran out sets a bit that pf_ops8_status reads. */
 

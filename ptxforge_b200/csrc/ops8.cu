@@ -28,6 +28,7 @@ using pf::DeviceGuard;
 typedef __nv_bfloat16 bf16;
 
 constexpr int kMaxDevices = 64;
+constexpr int kMostSize = 1 << 30;  // rows, columns, M, N, K: index arithmetic in 32 bits stays below 2^31
 constexpr unsigned long long kWaitNs = 4000000000ull;  // bound of each device-side wait
 constexpr int kMaxSumK = 131071;  // K * 128 * 128 stays below 2^31
 
@@ -351,6 +352,7 @@ Choice choose_one(const Device &d, int tokens, int channels, int sum, int elem, 
   const int kb = k_blocks_of(sum, elem);
   const double hbm = double(channels) * sum * elem / 6.7e6;
   for (int T = least_tokens; T <= 128; T *= 2) {
+    if (tokens > 65535ll * T) continue;  // the grid's second dimension
     const double tiles = std::ceil(channels / 128.0) * std::ceil(tokens / double(T));
     for (int S = 1; S <= 8 && kb >= 2 * S - 1; S *= 2) {
       const double ctas = std::ceil(tiles * S / d.num_sms), blocks = (kb + S - 1) / S;
@@ -522,11 +524,14 @@ int pf_quantize_s8(int device, pf_dtype src, int rows, int cols, const void *X, 
                    signed char *codes, long long ld_codes, float *scale, void *stream, char *err_text, size_t err_len) {
   const Err err{err_text, err_len};
   if (err_text && err_len) err_text[0] = '\0';
-  if (rows < 0 || cols < 0) return err(PF_EINVAL, "rows and cols must not be negative (got %d, %d)", rows, cols);
+  if (rows < 0 || cols < 0 || rows > kMostSize || cols > kMostSize)
+    return err(PF_EINVAL, "rows and cols must be 0 to 2^30 (got %d, %d)", rows, cols);
   if (src != PF_F32 && src != PF_BF16) return err(PF_EINVAL, "the source type must be f32 or bf16");
   if (axis != 0 && axis != 1) return err(PF_EINVAL, "axis must be 1 (a scale for each row) or 0 (for each column), got %d", axis);
-  if (rows == 0 || cols == 0) return PF_OK;
-  if (any_null(X, codes, scale)) return err(PF_EINVAL, "null argument");
+  const int lines = axis ? rows : cols;
+  if (lines == 0) return PF_OK;
+  const bool no_values = rows == 0 || cols == 0;  // each line's scale is the least one
+  if (any_null(scale) || (!no_values && any_null(X, codes))) return err(PF_EINVAL, "null argument");
   if (ldx < cols || ld_codes < cols) return err(PF_EINVAL, "a row stride is below cols");
   Device *d;
   cudaStream_t s;
@@ -534,6 +539,10 @@ int pf_quantize_s8(int device, pf_dtype src, int rows, int cols, const void *X, 
   if ((rc = device_of(device, err, &d))) return rc;
   DeviceGuard g(device);
   if ((rc = stream_of(device, stream, err, &s))) return rc;
+  if (no_values) {
+    pf::launch_pdl(&pf::least_scales, dim3(blocks_of(lines, 256)), 256, 0, s, scale, lines);
+    return launched(err);
+  }
   int8_t *q = reinterpret_cast<int8_t *>(codes);
   rc = src == PF_F32 ? quantize<float>(*d, X, ldx, rows, cols, axis, q, ld_codes, scale, s, err)
                      : quantize<bf16>(*d, X, ldx, rows, cols, axis, q, ld_codes, scale, s, err);
@@ -544,7 +553,8 @@ int pf_dequantize_s8(int device, int rows, int cols, const signed char *codes, l
                      int axis, pf_dtype dst, void *X, long long ldx, void *stream, char *err_text, size_t err_len) {
   const Err err{err_text, err_len};
   if (err_text && err_len) err_text[0] = '\0';
-  if (rows < 0 || cols < 0) return err(PF_EINVAL, "rows and cols must not be negative (got %d, %d)", rows, cols);
+  if (rows < 0 || cols < 0 || rows > kMostSize || cols > kMostSize)
+    return err(PF_EINVAL, "rows and cols must be 0 to 2^30 (got %d, %d)", rows, cols);
   if (dst != PF_F32 && dst != PF_BF16) return err(PF_EINVAL, "the destination type must be f32 or bf16");
   if (axis != 0 && axis != 1) return err(PF_EINVAL, "axis must be 1 (a scale for each row) or 0 (for each column), got %d", axis);
   if (rows == 0 || cols == 0) return PF_OK;
@@ -572,7 +582,7 @@ int pf_gemm_s8(int device, int M, int N, int K, const signed char *A, long long 
                long long ldc, void *workspace, size_t workspace_bytes, void *stream, char *err_text, size_t err_len) {
   const Err err{err_text, err_len};
   if (err_text && err_len) err_text[0] = '\0';
-  if (M < 0 || N < 0) return err(PF_EINVAL, "M and N must not be negative (got %d, %d)", M, N);
+  if (M < 0 || N < 0 || M > kMostSize || N > kMostSize) return err(PF_EINVAL, "M and N must be 0 to 2^30 (got %d, %d)", M, N);
   if (K < 1 || K > kMaxSumK)
     return err(PF_EINVAL, "K must be 1 to %d, so that a sum of int8 products fits 32 bits (got %d)", kMaxSumK, K);
   if (out != PF_F32 && out != PF_BF16) return err(PF_EINVAL, "the output type must be f32 or bf16");
@@ -614,7 +624,8 @@ int pf_gemm_bias_gelu_checkpoint(int device, int M, int N, int K, const void *A,
                                  char *err_text, size_t err_len) {
   const Err err{err_text, err_len};
   if (err_text && err_len) err_text[0] = '\0';
-  if (M < 0 || N < 1 || K < 1) return err(PF_EINVAL, "M must not be negative, N and K positive (got %d, %d, %d)", M, N, K);
+  if (M < 0 || N < 1 || K < 1 || M > kMostSize || N > kMostSize || K > kMostSize)
+    return err(PF_EINVAL, "M must be 0 to 2^30, N and K 1 to 2^30 (got %d, %d, %d)", M, N, K);
   if (N % 8 || K % 8) return err(PF_ESHAPE, "rows of A, B and C must be multiples of 16 bytes (N=%d, K=%d)", N, K);
   if (M == 0) return PF_OK;
   if (any_null(A, B, C) || any_null(bias) || any_null(grad_codes)) return err(PF_EINVAL, "null argument");
@@ -633,7 +644,7 @@ int pf_gemm_bias_gelu_checkpoint(int device, int M, int N, int K, const void *A,
 }
 
 size_t pf_gemm_bias_gelu_backward_workspace(int M, int N, int K) {
-  return M < 1 || N < 1 || K < 1 ? 0 : BackwardSpace(M, N, K).total;
+  return M < 1 || N < 1 || K < 1 || M > kMostSize || N > kMostSize || K > kMostSize ? 0 : BackwardSpace(M, N, K).total;
 }
 
 int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, const void *B, const signed char *a_codes,
@@ -641,7 +652,8 @@ int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, 
                                void *workspace, size_t workspace_bytes, void *stream, char *err_text, size_t err_len) {
   const Err err{err_text, err_len};
   if (err_text && err_len) err_text[0] = '\0';
-  if (M < 0 || N < 1 || K < 1) return err(PF_EINVAL, "M must not be negative, N and K positive (got %d, %d, %d)", M, N, K);
+  if (M < 0 || N < 1 || K < 1 || M > kMostSize || N > kMostSize || K > kMostSize)
+    return err(PF_EINVAL, "M must be 0 to 2^30, N and K 1 to 2^30 (got %d, %d, %d)", M, N, K);
   if (N % 8 || K % 8) return err(PF_ESHAPE, "rows of dC, B and the gradients must be multiples of 16 bytes (N=%d, K=%d)", N, K);
   Device *d;
   cudaStream_t s;

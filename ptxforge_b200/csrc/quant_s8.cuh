@@ -410,6 +410,13 @@ __global__ void __launch_bounds__(256) codes_cols_s8(const T *X, long long ldx, 
     store_codes<T, kVec, false>(y, s, inv, bad, Q + r * ldq + c);
   }
 }
+// Scales of rows (columns) that hold nothing.
+__global__ void __launch_bounds__(256) least_scales(float *scale, int n) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) scale[i] = kLeastScale;
+}
 __global__ void __launch_bounds__(256) scales_of_bits(uint32_t *amax, int n) {
   grid_launch_dependents();
   grid_dependency_wait();

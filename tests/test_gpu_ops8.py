@@ -72,6 +72,23 @@ def test_store(rows, cols, dtype, axis):
         assert torch.equal(back, (codes.float() * scale.unsqueeze(axis)).to(out))
 
 
+@pytest.mark.parametrize("rows", [5000, 4096])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_store_with_unaligned_scales(rows, dtype):
+    """Scales that start anywhere: no wide load of them fits."""
+    x = randn(rows, 136, seed=rows, dtype=dtype)
+    for axis in (1, 0):
+        want, want_scale = codes64(x, axis)
+        for first in (1, 2, 3):
+            room = torch.zeros(rows + 8, device=DEV)
+            s = room[first:first + want_scale.numel()]
+            codes, scale = pf.quantize_s8(x, axis, scale=s)
+            assert scale.data_ptr() == s.data_ptr() and torch.equal(codes, want) and torch.equal(s, want_scale)
+            assert torch.equal(pf.dequantize_s8(codes, s, axis, dtype=dtype), (want.float() * s.unsqueeze(axis)).to(dtype))
+            s.zero_()
+            assert not room.any()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("axis", [1, 0])
 @pytest.mark.parametrize("first,cols", [(3, 40), (8, 64), (1, 33), (0, 96)])
@@ -151,7 +168,9 @@ def check_s8(c, a, b, sa, sb, bias, gelu):
 
 PRODUCTS = [(1, 16, 16), (1, 1, 1), (1, 512, 4096), (3, 5, 7), (8, 256, 512), (17, 272, 528), (37, 512, 1040), (64, 64, 2048),
             (127, 129, 131), (128, 128, 128), (129, 256, 144), (200, 136, 80), (256, 256, 256), (300, 1008, 96),
-            (333, 1001, 2050), (1000, 1040, 528), (2050, 2064, 272), (5, 4100, 33)]
+            (333, 1001, 2050), (1000, 1040, 528), (2050, 2064, 272), (5, 4100, 33),
+            (24, 64, 4096), (40, 128, 8192), (100, 384, 8192), (256, 2048, 4096),  # split sums, of few and many tokens
+            (2500, 2048, 1040), (2500, 2049, 1030)]                                # pairs, and a last wave of single CTAs
 
 
 @pytest.mark.parametrize("M,N,K", PRODUCTS)
@@ -201,7 +220,8 @@ def test_product_of_a_token_with_a_nan_scale_is_nan_there_alone():
 # the product with an 8-bit checkpoint, and its gradients
 # ---------------------------------------------------------------------------------------------
 LAYERS = [(1, 8, 8), (1, 136, 72), (7, 64, 256), (77, 512, 512), (128, 128, 64), (129, 264, 136), (200, 136, 72),
-          (256, 256, 256), (300, 1024, 520), (515, 776, 1032), (1000, 72, 2048), (2100, 2056, 264), (1601, 1544, 1288)]
+          (256, 256, 256), (300, 1024, 520), (515, 776, 1032), (1000, 72, 2048), (2100, 2056, 264), (1601, 1544, 1288),
+          (2500, 2304, 2048), (20, 4096, 1024), (60, 256, 4096)]
 
 
 def layer(M, N, K, seed=0):
@@ -372,6 +392,9 @@ def test_no_tokens():
     assert q.shape == (0, 16) and s.shape == (0,) and pf.dequantize_s8(q, s).shape == (0, 16)
     b8, sb = pf.quantize_s8(b, axis=0)
     assert pf.gemm_s8(q, b8, s, sb, bias).shape == (0, 24)
+    # scales over nothing are the least one
+    assert (pf.quantize_s8(a, axis=0)[1] == TINY).all()
+    assert (pf.quantize_s8(b[:, :0], axis=1)[1] == TINY).all() and pf.quantize_s8(b[:, :0], axis=0)[1].shape == (0,)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -426,6 +449,66 @@ def test_a_trained_layer_captured_and_replayed():
         torch.cuda.synchronize()
         for ops, got in zip(held, outs):
             assert all(torch.equal(x, y) for x, y in zip(got, step(*ops)))
+
+
+def test_a_kernel_captured_at_its_first_use():
+    """A capture may be the first call of a size, and so of a kernel, once the device was set up by any other call."""
+    import subprocess
+    import sys
+    code = """
+import torch, ptxforge_b200 as pf
+x = torch.ones(2, 8, device="cuda")
+pf.quantize_s8(x)
+torch.cuda.synchronize()
+a = torch.randint(-127, 128, (700, 1040), dtype=torch.int8, device="cuda")
+b = torch.randint(-127, 128, (1040, 2064), dtype=torch.int8, device="cuda")
+s, t = torch.ones(700, device="cuda"), torch.ones(2064, device="cuda")
+h, w, bias = torch.randn(333, 264, device="cuda").bfloat16(), torch.randn(264, 520, device="cuda").bfloat16(), torch.randn(520, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    c = pf.gemm_s8(a, b, s, t, dtype=torch.float32)
+    d = pf.gemm_s8(a[:3], b, s[:3], t, dtype=torch.float32)
+    y, saved = pf.gemm_bias_gelu_checkpoint(h, w, bias)
+    grads = pf.gemm_bias_gelu_backward(y, w, saved)
+    q = pf.quantize_s8(w, axis=0)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(c, (a.double() @ b.double()).float()) and torch.equal(d, c[:3])
+y2, saved2 = pf.gemm_bias_gelu_checkpoint(h, w, bias)
+assert torch.equal(y, y2) and all(torch.equal(p, r) for p, r in zip(grads, pf.gemm_bias_gelu_backward(y2, w, saved2)))
+assert torch.equal(q[0], pf.quantize_s8(w, axis=0)[0]) and pf.ops8_status() == 0
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_of_two_threads():
+    """Two host threads, a stream each, products of the same weights: the library keeps nothing that they could share."""
+    import threading
+    a, b, bias = layer(300, 1032, 520)
+    g = randn(300, 1032, seed=3, dtype=torch.bfloat16)
+    c0, saved0 = pf.gemm_bias_gelu_checkpoint(a, b, bias)
+    want = (c0, *pf.gemm_bias_gelu_backward(g, b, saved0))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(30):
+                c, saved = pf.gemm_bias_gelu_checkpoint(a, b, bias)
+                got = (c, *pf.gemm_bias_gelu_backward(g, b, saved))
+                s.synchronize()
+                if not all(torch.equal(x, y) for x, y in zip(want, got)):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_a_stream_of_its_own():

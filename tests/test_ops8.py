@@ -40,18 +40,19 @@ def forward(M=4, N=8, K=16, a=P, b=P, bias=P, c=P, q=P, s=P, d=P):
 
 @pytest.mark.parametrize("got,code,needle", [
     (lambda: quantize(src=3), pf.PF_EINVAL, "f32 or bf16"),
-    (lambda: quantize(rows=-1), pf.PF_EINVAL, "negative"),
+    (lambda: quantize(rows=-1), pf.PF_EINVAL, "0 to 2^30"),
+    (lambda: quantize(rows=(1 << 30) + 1), pf.PF_EINVAL, "0 to 2^30"),
     (lambda: quantize(axis=2), pf.PF_EINVAL, "axis"),
     (lambda: quantize(x=None), pf.PF_EINVAL, "null"),
     (lambda: quantize(s=None), pf.PF_EINVAL, "null"),
     (lambda: quantize(ldx=7), pf.PF_EINVAL, "stride"),
     (lambda: quantize(ldq=7), pf.PF_EINVAL, "stride"),
     (lambda: dequantize(dst=1), pf.PF_EINVAL, "f32 or bf16"),
-    (lambda: dequantize(cols=-2), pf.PF_EINVAL, "negative"),
+    (lambda: dequantize(cols=-2), pf.PF_EINVAL, "0 to 2^30"),
     (lambda: dequantize(axis=-1), pf.PF_EINVAL, "axis"),
     (lambda: dequantize(q=None), pf.PF_EINVAL, "null"),
     (lambda: dequantize(ldx=3), pf.PF_EINVAL, "stride"),
-    (lambda: gemm(M=-1), pf.PF_EINVAL, "negative"),
+    (lambda: gemm(M=-1), pf.PF_EINVAL, "0 to 2^30"),
     (lambda: gemm(K=0), pf.PF_EINVAL, "K must be"),
     (lambda: gemm(K=131072, lda=131072), pf.PF_EINVAL, "131071"),
     (lambda: gemm(out=0 + 1), pf.PF_EINVAL, "f32 or bf16"),
@@ -61,7 +62,8 @@ def forward(M=4, N=8, K=16, a=P, b=P, bias=P, c=P, q=P, s=P, d=P):
     (lambda: gemm(sb=None), pf.PF_EINVAL, "null"),
     (lambda: gemm(), pf.PF_EINVAL, "workspace"),         # rows of B are 8 bytes
     (lambda: unaligned(), pf.PF_EINVAL, "workspace holds 100 bytes"),
-    (lambda: forward(N=0), pf.PF_EINVAL, "positive"),
+    (lambda: forward(N=0), pf.PF_EINVAL, "1 to 2^30"),
+    (lambda: forward(M=2 ** 31 - 1), pf.PF_EINVAL, "0 to 2^30"),
     (lambda: forward(N=12), pf.PF_ESHAPE, "16 bytes"),
     (lambda: forward(K=20), pf.PF_ESHAPE, "16 bytes"),
     (lambda: forward(d=None), pf.PF_EINVAL, "null"),
