@@ -548,12 +548,12 @@ struct NoJob {
   static constexpr bool kNone = true;
 };
 
-template <class J, int kStages>
+template <class J, int kStages, int kEpiWarps>
 struct PairConfig {
   typedef typename J::Operands Op;
   static constexpr int STAGES = kStages;
-  static constexpr int EPI_WARPS = 8;    // two to a quarter of the TMEM lanes, each with half of the tokens
-  static constexpr int EPI_BLOCKS = 4;   // blocks of 32 tokens a warp
+  static constexpr int EPI_WARPS = kEpiWarps;            // 8 or 16: 2 or 4 to a quarter of the TMEM lanes, which share its tokens
+  static constexpr int EPI_BLOCKS = 32 / EPI_WARPS;      // blocks of 32 tokens a warp
   static constexpr int THREADS = 64 + EPI_WARPS * 32;
   static constexpr int NUM_BARS = 2 * STAGES + 4 + 1;
   static constexpr int SMEM_BYTES = 1024 + STAGES * Op::STAGE_BYTES + NUM_BARS * 8 + 16;
@@ -561,12 +561,12 @@ struct PairConfig {
   static_assert(SMEM_BYTES <= 232448, "shared memory per block exceeds the sm_100 opt-in limit");
 };
 
-template <int kStages, class J1, class J2>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<J1, kStages>::THREADS, 1)
+template <int kStages, int kEpiWarps, class J1, class J2>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<J1, kStages, kEpiWarps>::THREADS, 1)
     gemm8_pair(const __grid_constant__ CUtensorMap tmW1, const __grid_constant__ CUtensorMap tmT1,
                const __grid_constant__ CUtensorMap tmW2, const __grid_constant__ CUtensorMap tmT2, const Gemm8Params p1,
                const Gemm8Params p2, const typename J1::Args args1, const typename J2::Args args2) {
-  using Cfg = PairConfig<J1, kStages>;
+  using Cfg = PairConfig<J1, kStages, kEpiWarps>;
   constexpr int W_BYTES = Cfg::Op::W_BYTES, T_BYTES = Cfg::Op::T_BYTES, STAGE_BYTES = Cfg::Op::STAGE_BYTES;
   __shared__ __align__(16) float scalars[Cfg::EPI_WARPS][Cfg::EPI_BLOCKS * 32];
   extern __shared__ uint8_t smem_raw[];
@@ -722,7 +722,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<J1, kStag
   } else {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int q = warp & 3, first = ((warp - 2) >> 2) * Cfg::EPI_BLOCKS * 32;
     float *mine = scalars[warp - 2];
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -730,7 +730,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<J1, kStag
       using Epi = typename decltype(job)::Epilogue;
       int ct, tt;
       pair_tile(i, p, ct, tt);
-      const int t0 = tt * 256 + half * 128;
+      const int t0 = tt * 256 + first;
       // what belongs to the channel and the tokens is loaded while the accumulator fills
       const Epi epi(args, ct * 256 + static_cast<int>(rank) * 128 + q * 32 + lane, p.channels);
       stage_scalars<Epi>(args, t0, Cfg::EPI_BLOCKS, p.tokens, lane, mine);
@@ -740,7 +740,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairConfig<J1, kStag
         return false;
       }
       tc_fence_after();
-      const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256 + half * 128);
+      const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * 256 + first);
       // The next block's sums travel from TMEM while this block's values are computed.
       uint32_t v[2][32];
       tmem_ld_32x32b_x32(t_row, v[0]);

@@ -452,22 +452,17 @@ struct PairJob {
 // tiles (a rectangle: the last token columns of the raster's last group) go to the one-CTA kernel, which spreads them
 // over the whole GPU: dB of 4096 x 14336 from 8192 tokens, 896 tiles on 74 pairs: 826 us in whole waves, 651 so.
 // `first`: a product whose tiles come before `last`'s, or null.
-template <class First, class Last>
-int run_pair(Device &d, First *first, Last &last, cudaStream_t s, const Err &err) {
+template <int kEpiWarps, class First, class Last>
+int run_pair_with(Device &d, First *first, Last &last, cudaStream_t s, const Err &err) {
   constexpr int kStages = 3;
   typedef typename Last::Kernel J;
-  using Cfg = pf::PairConfig<J, kStages>;
+  using Cfg = pf::PairConfig<J, kStages, kEpiWarps>;
   constexpr bool kTwo = !std::is_same<First, Last>::value;
-  int rc, units;
-  if ((rc = last.prepare(d, err))) return rc;
-  int before = 0;
-  if constexpr (kTwo) {
-    if ((rc = first->prepare(d, err))) return rc;
-    before = first->p.tiles;
-  }
+  const int before = kTwo ? first->p.tiles : 0;
   const void *func;
-  if constexpr (kTwo) func = reinterpret_cast<const void *>(&pf::gemm8_pair<kStages, typename First::Kernel, J>);
-  else func = reinterpret_cast<const void *>(&pf::gemm8_pair<kStages, J, pf::NoJob>);
+  if constexpr (kTwo) func = reinterpret_cast<const void *>(&pf::gemm8_pair<kStages, kEpiWarps, typename First::Kernel, J>);
+  else func = reinterpret_cast<const void *>(&pf::gemm8_pair<kStages, kEpiWarps, J, pf::NoJob>);
+  int rc, units;
   if ((rc = kernel_units(d, func, Cfg::SMEM_BYTES, Cfg::THREADS, err, &units))) return rc;
   pf::Gemm8Params &p = last.p;
   const int tiles = before + p.tiles, over = tiles % units, rows = p.c_tiles - (p.c_tiles - 1) / p.group * p.group;
@@ -476,15 +471,30 @@ int run_pair(Device &d, First *first, Last &last, cudaStream_t s, const Err &err
   p.tiles -= columns * rows;
   const dim3 grid(2 * std::min(tiles - columns * rows, units));
   if constexpr (kTwo)
-    pf::launch_pdl(&pf::gemm8_pair<kStages, typename First::Kernel, J>, grid, Cfg::THREADS, Cfg::SMEM_BYTES, s, first->w, first->t,
-                   last.w, last.t, first->p, p, first->args, last.args);
+    pf::launch_pdl(&pf::gemm8_pair<kStages, kEpiWarps, typename First::Kernel, J>, grid, Cfg::THREADS, Cfg::SMEM_BYTES, s, first->w,
+                   first->t, last.w, last.t, first->p, p, first->args, last.args);
   else
-    pf::launch_pdl(&pf::gemm8_pair<kStages, J, pf::NoJob>, grid, Cfg::THREADS, Cfg::SMEM_BYTES, s, last.w, last.t, last.w, last.t, p, p,
-                   last.args, pf::NoJob::Args{});
+    pf::launch_pdl(&pf::gemm8_pair<kStages, kEpiWarps, J, pf::NoJob>, grid, Cfg::THREADS, Cfg::SMEM_BYTES, s, last.w, last.t, last.w,
+                   last.t, p, p, last.args, pf::NoJob::Args{});
   if ((rc = launched(err)) || columns == 0) return rc;
   const int c0 = (p.c_tiles - rows) * 256, t0 = (p.t_tiles - columns) * 256;
   return run_best_one<Last::ELEM, Last::WK, Last::TK, typename Last::Epi>(d, last.g.template part<typename Last::Op>(c0, t0),
                                                                           last.args.part(c0, t0), s, err);
+}
+
+// 16 epilogue warps where the epilogue is what a launch waits for: few k-blocks a tile, or one or two tiles a pair, whose
+// last epilogue nothing covers.  8 otherwise: they take less power, which long launches run out of.  Measured, 8 / 16
+// warps, us: checkpoint 8192^2 x 1024 140 / 120, int8 with GELU 101 / 80, bf16 2048^3 21.4 / 19.9; sustained 16384 x 14336 x
+// 4096 checkpoint 1492 / 1526, int8 716 / 726.
+template <class First, class Last>
+int run_pair(Device &d, First *first, Last &last, cudaStream_t s, const Err &err) {
+  int rc;
+  if ((rc = last.prepare(d, err))) return rc;
+  if constexpr (!std::is_same<First, Last>::value)
+    if ((rc = first->prepare(d, err))) return rc;
+  const int tiles = last.p.tiles + (std::is_same<First, Last>::value ? 0 : first->p.tiles);
+  return k_blocks_of(last.g.sum, Last::ELEM) < 32 || tiles <= d.num_sms ? run_pair_with<16>(d, first, last, s, err)
+                                                                        : run_pair_with<8>(d, first, last, s, err);
 }
 
 // Elements, W's and T's order, epilogue -> the kernel for the sizes.
