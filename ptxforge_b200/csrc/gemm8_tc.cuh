@@ -320,7 +320,7 @@ __device__ __forceinline__ void put_block(const Epi &e, const uint32_t (&v)[N], 
 // one CTA a tile, the sum split over a cluster
 // ------------------------------------------------------------------------------------------------
 constexpr int kOneThreads = 192;
-constexpr int kOneMaxStages = 16;
+constexpr int kOneMaxStages = 8;
 
 // This CTA's share of the tokens: every CTA's sums, added in rank order.  They lie as [token][128 channels]; a warp takes a
 // token, a lane four of its channels, so that what crosses between SMs are whole lines (as [channel][token], 16 bytes a

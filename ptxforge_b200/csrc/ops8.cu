@@ -179,7 +179,8 @@ void quantize_rows(const T *x, long long ldx, int rows, int cols, int8_t *q, lon
 }
 
 // Strips of whole columns held in shared memory: 512 rows of 128 bytes a CTA, so that three CTAs share an SM, one's loads
-// beside another's stores.
+// beside another's stores.  What bounds it is that memory: a CTA's chain (load, maximum, exchange, codes) takes 10 us, and
+// 192 KB an SM over 10 us are 2.8 TB/s.  4096 x 14336 fp32: 80 us, 84 with 256 rows a CTA in clusters of 16.
 template <class T>
 int quantize_strips(Device &d, const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale,
                     cudaStream_t s, const Err &err) {
@@ -396,11 +397,14 @@ int run_one(Device &d, const Product &g, int splits, const typename Epi::Args &a
   p.status = d.status;
   p.timeout_ns = kWaitNs;
   const long long tiles = static_cast<long long>(p.c_tiles) * p.t_tiles;
-  // As deep a pipeline as lets the CTAs of one SM share its memory, at least what the split sums need.
+  // As deep a pipeline as lets the CTAs of one SM share its memory, at least what the split sums need; no deeper than
+  // keeps the memory busy, so that the next launch finds room to start beside the last CTAs (int8 1 x 14336 x 4096, two CTAs
+  // an SM: 6 stages 13.3 us, 4 12.9; 37 x 4096 x 14336, one: 6 14.4, 8 14.7).
   const int per_sm = static_cast<int>(std::min<long long>(4, (tiles * splits + d.num_sms - 1) / d.num_sms));
   const int room = (kSmemPerSm / per_sm - kOneStatic - 2048) / Op::STAGE_BYTES;  // alignment, and 1 KB of the system's
   const int least = std::max(2, (Op::TOKENS * 512 + Op::STAGE_BYTES - 1) / Op::STAGE_BYTES);
-  p.stages = std::max(least, std::min({room, pf::kOneMaxStages, (p.k_blocks + splits - 1) / splits}));
+  const int busy = per_sm == 1 ? 6 : per_sm == 2 ? 4 : 3;
+  p.stages = std::max(least, std::min({room, busy, (p.k_blocks + splits - 1) / splits}));
   pf::launch_cluster(&pf::gemm8_one<Op, Epi>, dim3(p.c_tiles * splits, p.t_tiles), dim3(pf::kOneThreads),
                      1024 + p.stages * Op::STAGE_BYTES, splits, s, w, t, p, args);
   return launched(err);
