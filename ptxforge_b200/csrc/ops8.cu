@@ -342,7 +342,7 @@ constexpr int kOneStatic = 3072;        // of gemm8_one: barriers and token scal
 //   pair: 0.28 a k-block and wave, 11.5 for the launch and the last epilogue.
 // Measured / by this rule, bf16, M x N x K: 1024 x 2048 x 8192 T128 S2 36 / 38, S1 50 / 51, pair 49 / 47;
 // 512 x 4096 x 4096 T128 S2 23 / 23, pair 30 / 29; 256 x 4096 x 4096 T128 S4 16 / 15, T64 S2 17 / 17; 1024^3 T64 S2 9.4 / 9.4;
-// 2048^3 pair 21 / 20, T128 S1 24 / 24.
+// 2048^3 pair 20 / 20, T128 S1 24 / 24.
 struct Choice {
   int tokens = 0, splits = 1;
   double us = 1e30;
@@ -528,7 +528,6 @@ int two_products(Device &d, const Product &ga, const typename EpiA::Args &aa, co
   const int rc = product<2, true, true, EpiA>(d, ga, aa, s, err);
   return rc ? rc : product<2, false, false, EpiB>(d, gb, ab, s, err);
 }
-
 
 }  // namespace
 

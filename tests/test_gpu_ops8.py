@@ -471,12 +471,15 @@ with torch.cuda.graph(g):
     y, saved = pf.gemm_bias_gelu_checkpoint(h, w, bias)
     grads = pf.gemm_bias_gelu_backward(y, w, saved)
     q = pf.quantize_s8(w, axis=0)
+    r = pf.quantize_s8(h[:, 1:], axis=0)   # unaligned: a memset and three kernels
+    none = pf.gemm_bias_gelu_backward(y[:0], w, pf.Checkpoint(saved.a_codes[:0], saved.a_scale[:0], saved.grad_codes[:0]))
 g.replay()
 torch.cuda.synchronize()
 assert torch.equal(c, (a.double() @ b.double()).float()) and torch.equal(d, c[:3])
 y2, saved2 = pf.gemm_bias_gelu_checkpoint(h, w, bias)
 assert torch.equal(y, y2) and all(torch.equal(p, r) for p, r in zip(grads, pf.gemm_bias_gelu_backward(y2, w, saved2)))
-assert torch.equal(q[0], pf.quantize_s8(w, axis=0)[0]) and pf.ops8_status() == 0
+assert all(torch.equal(p, t) for p, t in zip((*q, *r), (*pf.quantize_s8(w, axis=0), *pf.quantize_s8(h[:, 1:], axis=0))))
+assert not none[1].any() and not none[2].any() and pf.ops8_status() == 0
 print("captured")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
