@@ -258,9 +258,12 @@ void dequantize_grad(const unsigned char *codes, long long n, void *X, cudaStrea
   T *x = static_cast<T *>(X);
   constexpr int kVec = 16 / sizeof(T);
   const bool wide = reinterpret_cast<uintptr_t>(codes) % kVec == 0 && pf::aligned16(X);
-  const int per = 256 * (wide ? kVec : 1);
+  // Four vectors a thread where that leaves enough blocks (16384 x 14336 to bf16: 129 us with one, 105 with four), one below.
+  const bool ahead = wide && n >= 1024ll * 256 * 4 * kVec;
+  const int per = 256 * (wide ? kVec : 1) * (ahead ? 4 : 1);
   const dim3 grid(static_cast<unsigned>(std::min<long long>((n + per - 1) / per, 1 << 30)));
-  pf::launch_pdl(wide ? &pf::dequantize_grad<T, kVec> : &pf::dequantize_grad<T, 1>, grid, 256, 0, s, codes, n, x);
+  const auto kernel = ahead ? &pf::dequantize_grad<T, kVec, 4> : wide ? &pf::dequantize_grad<T, kVec, 1> : &pf::dequantize_grad<T, 1, 1>;
+  pf::launch_pdl(kernel, grid, 256, 0, s, codes, n, x);
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -271,9 +274,11 @@ struct BackwardSpace {
   int col_blocks, rows, parts;
   BackwardSpace(int M, int N, int K) {
     // 128 rows a block of the elementwise kernel (and a part of dbias' sums); 32 where that makes too few blocks to keep
-    // the memory busy (1999 x 2048: 6.8 us with 128, 5.3 with 32).
+    // the memory busy (1999 x 2048: 6.8 us with 128, 5.3 with 32, before a thread loaded four rows at
+    // once; 4.0 since).  Up to 128 tokens are one part, which needs no launch
+    // to join parts (a backward pass of 77 x 512 x 512 waits for its launches: 16.8 us with three parts, 14.4 with one).
     col_blocks = (N + pf::kDzCols - 1) / pf::kDzCols;
-    rows = (M + 127) / 128 * static_cast<long long>(col_blocks) < 1024 ? 32 : 128;
+    rows = M > 128 && (M + 127) / 128 * static_cast<long long>(col_blocks) < 1024 ? 32 : 128;
     parts = (M + rows - 1) / rows;
     dz = 0;
     a = dz + round256(size_t(M) * N * sizeof(bf16));

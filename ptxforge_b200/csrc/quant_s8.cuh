@@ -487,21 +487,30 @@ __global__ void __launch_bounds__(256) dequantize_s8(const int8_t *Q, long long 
   if (r < rows) restore_row<T, kVec, kByRow>(Q + r * ldq, cols, kByRow ? scale + r : scale, X + r * ldx, threadIdx.x, blockDim.x);
 }
 
-template <class T, int kVec>
+// kGradAhead vectors a thread, all on their way at once.
+template <class T, int kVec, int kGradAhead>
 __global__ void __launch_bounds__(256) dequantize_grad(const uint8_t *D, long long n, T *X) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const long long stride = static_cast<long long>(gridDim.x) * 256 * kVec;
-  for (long long i = (blockIdx.x * 256ll + threadIdx.x) * kVec; i < n; i += stride) {
-    if (kVec > 1 && i + kVec <= n) {
-      if constexpr (kVec > 1) {
-        float v[kVec];
-        load_codes(D + i, v, [](uint32_t w, float (&a)[4]) { grad_steps4(w, a); });
+  const long long stride = static_cast<long long>(gridDim.x) * 256 * kVec * kGradAhead;
+  for (long long base = blockIdx.x * (256ll * kVec * kGradAhead) + threadIdx.x * kVec; base < n; base += stride) {
+    if constexpr (kVec > 1) {
+      if (base + (kGradAhead - 1) * 256ll * kVec + kVec <= n) {
+        float v[kGradAhead][kVec];
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) v[j] = grad_value(v[j]);
-        store_vec(X + i, v);
+        for (int b = 0; b < kGradAhead; ++b)
+          load_codes(D + base + b * 256 * kVec, v[b], [](uint32_t w, float (&a)[4]) { grad_steps4(w, a); });
+#pragma unroll
+        for (int b = 0; b < kGradAhead; ++b) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) v[b][j] = grad_value(v[b][j]);
+          store_vec(X + base + b * 256 * kVec, v[b]);
+        }
+        continue;
       }
-    } else {
+    }
+    for (int b = 0; b < kGradAhead; ++b) {
+      const long long i = base + b * 256 * kVec;
       for (long long j = i; j < n && j < i + kVec; ++j) {
         float k[4];
         grad_steps4(D[j], k);
@@ -570,22 +579,35 @@ __global__ void __launch_bounds__(256) backward_operands(const __nv_bfloat16 *dC
   float sum[8] = {};
   if (c < N) {
     const int r0 = rb * dz_rows + row, r1 = min(M, (rb + 1) * dz_rows);
-#pragma unroll 4
-    for (int r = r0; r < r1; r += 8) {
-      const long long i = static_cast<long long>(r) * N + c;
-      const uint4 g = *reinterpret_cast<const uint4 *>(dC + i);
-      const float m = a_scale ? split_scale(__ldg(a_scale + r)).m : 1.f;
-      float k[8], v[8];
-      load_codes(D + i, k, [](uint32_t w, float (&a)[4]) { grad_steps4(w, a); });
-      const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+    for (int r = r0; r < r1; r += 32) {
+      // four rows on their way at once, the last ones too
+      uint4 g[4];
+      uint2 w[4];
+      float m[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = __uint_as_float((j & 1) ? gw[j / 2] & 0xFFFF0000u : gw[j / 2] << 16);
-        const float z = x * k[j] * (1.f / kGradSteps);
-        sum[j] += z;
-        v[j] = z * m;
+      for (int b = 0; b < 4; ++b) {
+        if (r + b * 8 >= r1) break;
+        const long long i = static_cast<long long>(r + b * 8) * N + c;
+        g[b] = *reinterpret_cast<const uint4 *>(dC + i);
+        w[b] = *reinterpret_cast<const uint2 *>(D + i);
+        m[b] = a_scale ? __ldg(a_scale + r + b * 8) : 1.f;
       }
-      store_vec(dz + i, v);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (r + b * 8 >= r1) break;
+        float k[8], v[8];
+        load_codes(&w[b], k, [](uint32_t x, float (&a)[4]) { grad_steps4(x, a); });
+        const float f = a_scale ? split_scale(m[b]).m : 1.f;
+        const uint32_t gw[4] = {g[b].x, g[b].y, g[b].z, g[b].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = __uint_as_float((j & 1) ? gw[j / 2] & 0xFFFF0000u : gw[j / 2] << 16);
+          const float z = x * k[j] * (1.f / kGradSteps);
+          sum[j] += z;
+          v[j] = z * f;
+        }
+        store_vec(dz + static_cast<long long>(r + b * 8) * N + c, v);
+      }
     }
   }
 #pragma unroll

@@ -277,6 +277,10 @@ def test_every_grad_code_stands_for_its_step():
     assert torch.equal(pf.dequantize_gelu_grad(codes[:255].clone()), want[:255].bfloat16())
     big = torch.randint(0, 253, (1003, 77), dtype=torch.uint8, device=DEV, generator=gen(1))
     assert torch.equal(pf.dequantize_gelu_grad(big, dtype=torch.float32), want[big.long()])
+    big = torch.randint(0, 253, (8192 * 1024 + 4333,), dtype=torch.uint8, device=DEV, generator=gen(2))
+    for part in (big, big[1:], big[:8192 * 1024 - 8]):  # four vectors a thread; codes that start anywhere; a whole last block less
+        for dtype in (torch.bfloat16, torch.float32):
+            assert torch.equal(pf.dequantize_gelu_grad(part, dtype=dtype), want[part.long()].to(dtype))
 
 
 def grads64(dc, b, saved):
