@@ -463,6 +463,8 @@ struct PairJob {
 // `first`: a product whose tiles come before `last`'s, or null.
 template <int kEpiWarps, class First, class Last>
 int run_pair_with(Device &d, First *first, Last &last, cudaStream_t s, const Err &err) {
+  // Stages of two 128-byte atoms of the sum; sustained 16384 x 14336 x 4096 checkpoint, us: 3 of two 1475, 6 of one 1565; 3 of two
+  // 1454, 2 of three 1600.
   constexpr int kStages = 3;
   typedef typename Last::Kernel J;
   using Cfg = pf::PairConfig<J, kStages, kEpiWarps>;
