@@ -338,7 +338,7 @@ int operand_maps(const Product &g, const Err &err, CUtensorMap *w, CUtensorMap *
 }
 
 constexpr int kSmemPerSm = 227 * 1024;  // of one SM, for the CTAs that share it
-constexpr int kOneStatic = 3072;        // of gemm8_one: barriers and token scalars
+constexpr int kOneStatic = 3 * 1024;    // of gemm8_one: barriers and token scalars
 
 // What a product costs, in us on a B200, by the measurements below; it is used to choose a kernel, never to skip work.
 //   one CTA, T tokens a tile, S splits: an SM takes in 92 KB/us of operands with one CTA, 130 with more (a k-block is 16 KB
