@@ -59,8 +59,8 @@ def dequantize_s8(codes, scale, axis: int = 1, out=None, *, dtype=None, stream=N
 def gemm_s8(A, B, scale_a, scale_b, bias=None, C=None, *, gelu: bool = False, dtype=None, stream=None):
     """C = f(scale_a[:, None] * scale_b * (A @ B) + bias), A [M, K] and B [K, N] int8 codes, scale_a float32 [M] (a
     scale for each token), scale_b float32 [N] (for each channel), bias float32 [N] or None; f is GELU's tanh form with
-    gelu=True, else the identity.  `dtype` of C: bfloat16 (default) or float32.  The integer sums are exact; K is at
-    most 131071.  Any M, N, K; row strides are free."""
+    gelu=True, else the identity.  `dtype` of C: bfloat16 (default) or float32.  The integer sums are exact, for
+    which K is 1 to 131071.  M and N are free, and so are row strides."""
     return _ops().gemm_s8(A, B, scale_a, scale_b, bias, C, gelu, dtype, _handle(stream))
 
 
