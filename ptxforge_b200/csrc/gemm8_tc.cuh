@@ -330,26 +330,33 @@ template <int kTokens, int kSplits, class Epi>
 __device__ __forceinline__ void join_sums(const typename Epi::Args &args, int c0, int channels, uint32_t base, uint32_t rank,
                                           int warp, int lane, int t0, int tokens, const float *scalars) {
   constexpr int SHARE = kTokens / kSplits, AHEAD = SHARE < 4 ? 1 : kSplits == 8 || SHARE < 16 ? 1 : kSplits == 4 ? 2 : 4;
+  static_assert(AHEAD == 1 || SHARE % (4 * AHEAD) == 0, "the look-ahead stays in this CTA's share");
   const typename Epi::Row row(args, c0 + lane * 4, channels);
+  const bool inside = c0 + lane * 4 < channels;
   const int mine = static_cast<int>(rank) * SHARE;
   uint32_t from[kSplits];
 #pragma unroll
   for (int s = 0; s < kSplits; ++s) from[s] = mapa_shared(base + lane * 16, s);
 #pragma unroll 1
   for (int t = mine + warp; t < mine + SHARE && t0 + t < tokens; t += 4 * AHEAD) {
+    // Only sums that are stored below: the cluster's last barrier orders no memory, so what makes a remote load end before
+    // its CTA may leave is that its value is used.
     uint32_t v[AHEAD][kSplits][4];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
+    for (int i = 0; i < AHEAD; ++i) {
+      if (!inside || t0 + t + i * 4 >= tokens) continue;
 #pragma unroll
       for (int s = 0; s < kSplits; ++s) ld_cluster<4>(from[s] + (t + i * 4) * 512, v[i][s]);
+    }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
+      const int at = t + i * 4;
+      if (!inside || t0 + at >= tokens) continue;
 #pragma unroll
       for (int s = 1; s < kSplits; ++s)
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[i][0][j] = Epi::add(v[i][0][j], v[i][s][j]);
-      const int at = t + i * 4;
-      if (t0 + at < tokens) row.put(v[i][0], t0 + at, Epi::kTokenScalar ? scalars[at] : 0.f);
+      row.put(v[i][0], t0 + at, Epi::kTokenScalar ? scalars[at] : 0.f);
     }
   }
 }
