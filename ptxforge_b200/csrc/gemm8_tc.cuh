@@ -101,7 +101,7 @@ __device__ __forceinline__ bool rows_of_four(const Out *out, long long ld) {
   return ld % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(Out)) == 0;
 }
 __device__ __forceinline__ float4 load_channels(const float *p, int n) {
-  return make_float4(n > 0 ? __ldg(p) : 0.f, n > 1 ? __ldg(p + 1) : 0.f, n > 2 ? __ldg(p + 2) : 0.f, n > 3 ? __ldg(p + 3) : 0.f);
+  return make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
 }
 
 template <class Out>
@@ -120,10 +120,10 @@ struct EpilogueS8 {
   float sb, bias;
   __device__ __forceinline__ EpilogueS8(const Args &args, int channel, int channels)
       : a(args), c(channel), inside(channel < channels) {
-    sb = inside ? __ldg(a.sb + c) : 0.f;
-    bias = inside && a.bias ? __ldg(a.bias + c) : 0.f;
+    sb = inside ? a.sb[c] : 0.f;
+    bias = inside && a.bias ? a.bias[c] : 0.f;
   }
-  static __device__ __forceinline__ float token(const Args &a, int t) { return __ldg(a.sa + t); }
+  static __device__ __forceinline__ float token(const Args &a, int t) { return a.sa[t]; }
   static __device__ __forceinline__ uint32_t add(uint32_t x, uint32_t y) { return x + y; }
   // Two tokens' sums and scalars -> their values.
   template <bool kGelu>
@@ -196,7 +196,7 @@ struct EpilogueCheckpoint : EpilogueF32Sum {
   float bias;
   __device__ __forceinline__ EpilogueCheckpoint(const Args &args, int channel, int channels)
       : a(args), c(channel), inside(channel < channels) {
-    bias = inside ? __ldg(a.bias + c) : 0.f;
+    bias = inside ? a.bias[c] : 0.f;
   }
   static __device__ __forceinline__ float token(const Args &, int) { return 0.f; }
   __device__ __forceinline__ void put(uint32_t sum, int t, float) const {
@@ -261,7 +261,7 @@ struct EpilogueBf16 : EpilogueF32Sum {
   __device__ __forceinline__ EpilogueBf16(const Args &args, int channel, int channels)
       : a(args), c(channel), inside(channel < channels) {}
   static __device__ __forceinline__ float token(const Args &a, int t) {
-    return kDivided ? __fdiv_rn(1.f, split_scale(__ldg(a.token_scale + t)).m) : 1.f;
+    return kDivided ? __fdiv_rn(1.f, split_scale(a.token_scale[t]).m) : 1.f;
   }
   __device__ __forceinline__ void put(uint32_t sum, int t, float inv_m) const {
     if (inside) a.out[t * a.ld + c] = __float2bfloat16_rn(__uint_as_float(sum) * (kDivided ? inv_m : 1.f));

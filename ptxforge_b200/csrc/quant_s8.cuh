@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(256) codes_cols_s8(const T *X, long long ldx, 
   bool bad = false;
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
-    s[j] = scale_of(__ldg(amax + c + j)), inv[j] = __fdiv_rn(1.f, s[j]);
+    s[j] = scale_of(amax[c + j]), inv[j] = __fdiv_rn(1.f, s[j]);
     bad |= s[j] != s[j];
   }
 #pragma unroll 4
@@ -452,7 +452,7 @@ __device__ __forceinline__ void load_codes(const void *p, float (&q)[kVec], Four
 // kVec: 16 bytes of values, or 1.  blockDim.x threads a row, blockDim.y rows a block.
 template <class T, int kVec, bool kByRow, bool kInput = false>
 __device__ __forceinline__ void restore_row(const int8_t *q, int cols, const float *scale, T *x, int first, int step) {
-  float s = kByRow ? __ldg(scale) : 0.f;
+  float s = kByRow ? *scale : 0.f;
   if constexpr (kInput) s = split_scale(s).e;
   if constexpr (kVec > 1) {
 #pragma unroll 4
@@ -465,17 +465,17 @@ __device__ __forceinline__ void restore_row(const int8_t *q, int cols, const flo
       } else if ((reinterpret_cast<uintptr_t>(scale) & 15) == 0) {
 #pragma unroll
         for (int j = 0; j < kVec; j += 4) {
-          const float4 a = __ldg(reinterpret_cast<const float4 *>(scale + c + j));
+          const float4 a = *reinterpret_cast<const float4 *>(scale + c + j);
           v[j] *= a.x, v[j + 1] *= a.y, v[j + 2] *= a.z, v[j + 3] *= a.w;
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) v[j] *= __ldg(scale + c + j);
+        for (int j = 0; j < kVec; ++j) v[j] *= scale[c + j];
       }
       store_vec(x + c, v);
     }
   } else {
-    for (int c = first; c < cols; c += step) x[c] = from_f32<T>(static_cast<float>(q[c]) * (kByRow ? s : __ldg(scale + c)));
+    for (int c = first; c < cols; c += step) x[c] = from_f32<T>(static_cast<float>(q[c]) * (kByRow ? s : scale[c]));
   }
 }
 template <class T, int kVec, bool kByRow>
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(128) align_rows(const AlignRows a, const Align
   for (int i = threadIdx.x; i * 16 < cols; i += blockDim.x) {
     uint32_t v[5];
 #pragma unroll
-    for (int j = 0; j < 5; ++j) v[j] = i * 4 + j < words ? __ldg(x + i * 4 + j) : 0u;
+    for (int j = 0; j < 5; ++j) v[j] = i * 4 + j < words ? x[i * 4 + j] : 0u;
     Y[r * ld_y + i] = make_uint4(__funnelshift_r(v[0], v[1], shift), __funnelshift_r(v[1], v[2], shift),
                                  __funnelshift_r(v[2], v[3], shift), __funnelshift_r(v[3], v[4], shift));
   }
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(256) backward_operands(const __nv_bfloat16 *dC
         const long long i = static_cast<long long>(r + b * 8) * N + c;
         g[b] = *reinterpret_cast<const uint4 *>(dC + i);
         w[b] = *reinterpret_cast<const uint2 *>(D + i);
-        m[b] = a_scale ? __ldg(a_scale + r + b * 8) : 1.f;
+        m[b] = a_scale ? a_scale[r + b * 8] : 1.f;
       }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {

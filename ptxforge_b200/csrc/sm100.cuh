@@ -218,6 +218,8 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 // memory is visible (returns at once for a launch without the programmatic attribute).  grid_launch_dependents:
 // a dependent launched with that attribute may be scheduled once every CTA of this grid has signalled (or
 // exited); it still waits for this grid's completion before touching memory.
+// What an earlier launch may have written is read by ordinary loads alone: a non-coherent one (the read-only path) wants
+// its data unchanged for the whole life of the kernel, which here begins before the writer has ended.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" :::); }
 

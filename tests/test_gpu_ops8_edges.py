@@ -56,3 +56,52 @@ def test_split_sums_of_gradients_of_any_number_of_tokens(N, K):
         for need in (("dA",), ("dA", "dB")):
             got = pf.gemm_bias_gelu_backward(dc[:M], b, part, need=need)[0]
             within(got, want[:M], tol[:M] + BF * (want[:M].abs() + tol[:M]))
+
+
+# ---------------------------------------------------------------------------------------------
+# kernels that start before the one that writes their operands has ended
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("M,D,H", [(3, 264, 520), (300, 1024, 2056), (2500, 264, 2056), (90, 1001, 777)])
+def test_a_chain_through_the_same_buffers_reads_what_the_last_launch_wrote(M, D, H):
+    """Codes, scales, bias and results of 40 steps go through one set of buffers with no wait between them; every step gives
+    the bits of the same calls made one at a time, with the GPU waited for after each."""
+    xs = [randn(M, D, seed=i, dtype=torch.bfloat16) * (1 + i) for i in range(40)]
+    w8, sw = pf.quantize_s8(randn(D, H, seed=99), axis=0)
+    bias8 = torch.randint(-127, 128, (1, H), dtype=torch.int8, device=DEV)
+    q, s = torch.empty(M, D, dtype=torch.int8, device=DEV), torch.empty(M, device=DEV)
+    bias, one = torch.empty(1, H, device=DEV), torch.empty(1, device=DEV)
+    h = torch.empty(M, H, dtype=torch.bfloat16, device=DEV)
+    hq, hs = torch.empty(M, H, dtype=torch.int8, device=DEV), torch.empty(H, device=DEV)
+    steps = [torch.full((1,), 0.01 * (1 + i), device=DEV) for i in range(40)]
+
+    def step(i, wait):
+        out = torch.empty(M, H, device=DEV)
+        for call in (lambda: pf.quantize_s8(xs[i], codes=q, scale=s),
+                     lambda: pf.dequantize_s8(bias8, steps[i], out=bias),
+                     lambda: pf.gemm_s8(q, w8, s, sw, bias[0], h, gelu=True),
+                     lambda: pf.quantize_s8(h, 0, codes=hq, scale=hs),
+                     lambda: pf.dequantize_s8(hq, hs, 0, out=out)):
+            call()
+            if wait:
+                torch.cuda.synchronize()
+        return out
+
+    want = [step(i, True) for i in range(40)]
+    got = [step(i, False) for i in range(40)]
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+def test_a_backward_pass_reads_the_checkpoint_that_was_just_written():
+    M, N, K = 300, 1032, 520
+    a, b, bias = layer(M, N, K)
+    xs = [randn(M, K, seed=i, dtype=torch.bfloat16) * (1 + i) for i in range(30)]
+
+    def step(x, wait):
+        c, saved = pf.gemm_bias_gelu_checkpoint(x, b, bias)
+        if wait:
+            torch.cuda.synchronize()
+        return (c, *pf.gemm_bias_gelu_backward(c, b, saved))
+
+    want = [step(x, True) for x in xs]
+    got = [step(x, False) for x in xs]
+    assert all(torch.equal(p, r) for x, y in zip(want, got) for p, r in zip(x, y))
