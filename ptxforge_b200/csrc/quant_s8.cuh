@@ -70,13 +70,17 @@ __device__ __forceinline__ SplitScale split_scale(float s) {
   return {__uint_as_float((b & 0x007FFFFFu) | 0x3F800000u), __uint_as_float(b & 0xFF800000u)};
 }
 
-// The whole numbers that four codes in a word stand for: grad codes code - 26 (NaN for 255), or int8 codes.  A byte put
-// under the exponent of 2^23 is the float 2^23 + byte.
+// The whole numbers that four codes in a word stand for: grad codes code - 26 (NaN for 255) in steps of 1 or of 1 / 256,
+// or int8 codes.  A byte put under the exponent of 2^23 is the float 2^23 + byte, under that of 2^15 2^15 + byte / 256.
+constexpr float kGradUnit = 1.f / 256;
+template <bool kInUnits = false>
 __device__ __forceinline__ void grad_steps4(uint32_t w, float (&k)[4]) {
+  constexpr float UNIT = kInUnits ? kGradUnit : 1.f;
+  constexpr uint32_t BASE = kInUnits ? 0x47000000u : 0x4B000000u;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t b = __byte_perm(w, 0x4B000000u, 0x7650 | j);
-    k[j] = b == (0x4B000000u | kGradNan) ? __uint_as_float(0x7FC00000u) : __uint_as_float(b) - (8388608.f + kGradZero);
+    const uint32_t b = __byte_perm(w, BASE, 0x7650 | j);
+    k[j] = b == (BASE | kGradNan) ? __uint_as_float(0x7FC00000u) : __uint_as_float(b) - (8388608.f + kGradZero) * UNIT;
   }
 }
 __device__ __forceinline__ void codes4(uint32_t w, float (&q)[4]) {
@@ -557,9 +561,9 @@ __global__ void __launch_bounds__(128) align_rows(const AlignRows a, const Align
 // the backward pass's elementwise part
 // ------------------------------------------------------------------------------------------------
 // Blocks below dz_blocks: m dz = m dC d~ (rounded once to bf16) of 256 columns x dz_rows rows and, from the unrounded dz,
-// their column sums in fp32 (`sums` [row block][column]; with one row block that is dbias).  dC k is exact in fp32 (8 by
-// 8 bits), so dz is rounded once by 1 / 200.  The blocks after them: the input's q 2^e in bf16, exact, a row each.
-// a_scale may be null (m = 1, no input wanted).
+// their column sums in fp32 (`sums` [row block][column]; with one row block that is dbias).  dC k / 256 is exact in fp32 (8
+// by 8 bits) and finite where dC is, which dC k is not; so dz is rounded once, by 256 / 200.  The blocks after them: the
+// input's q 2^e in bf16, exact, a row each.  a_scale may be null (m = 1, no input wanted).
 constexpr int kDzCols = 256;
 __global__ void __launch_bounds__(256) backward_operands(const __nv_bfloat16 *dC, const uint8_t *D, const float *a_scale,
                                                          int M, int N, int dz_blocks, int col_blocks, int dz_rows,
@@ -596,13 +600,13 @@ __global__ void __launch_bounds__(256) backward_operands(const __nv_bfloat16 *dC
       for (int b = 0; b < 4; ++b) {
         if (r + b * 8 >= r1) break;
         float k[8], v[8];
-        load_codes(&w[b], k, [](uint32_t x, float (&a)[4]) { grad_steps4(x, a); });
+        load_codes(&w[b], k, [](uint32_t x, float (&a)[4]) { grad_steps4<true>(x, a); });
         const float f = a_scale ? split_scale(m[b]).m : 1.f;
         const uint32_t gw[4] = {g[b].x, g[b].y, g[b].z, g[b].w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float x = __uint_as_float((j & 1) ? gw[j / 2] & 0xFFFF0000u : gw[j / 2] << 16);
-          const float z = x * k[j] * (1.f / kGradSteps);
+          const float z = x * k[j] * (1.f / kGradUnit / kGradSteps);
           sum[j] += z;
           v[j] = z * f;
         }

@@ -105,3 +105,36 @@ def test_a_backward_pass_reads_the_checkpoint_that_was_just_written():
     want = [step(x, True) for x in xs]
     got = [step(x, False) for x in xs]
     assert all(torch.equal(p, r) for x, y in zip(want, got) for p, r in zip(x, y))
+
+
+# ---------------------------------------------------------------------------------------------
+# values near the ends of their types' ranges
+# ---------------------------------------------------------------------------------------------
+def check_backward(dc, b, saved):
+    """All three gradients within the tolerances of test_gpu_ops8.test_backward."""
+    (M, N), K = dc.shape, b.shape[0]
+    dz, a, want_a, want_b, want_bias = grads64(dc, b, saved)
+    dA, dB, dbias = pf.gemm_bias_gelu_backward(dc, b, saved)
+    tol = (BF + (N + 2) * 2.0 ** -23) * (dz.abs() @ b.double().abs().t())
+    within(dA, want_a, tol + BF * (want_a.abs() + tol))
+    tol = (BF + (M + 3) * 2.0 ** -23) * (a.abs().t() @ dz.abs())
+    within(dB, want_b, tol + BF * (want_b.abs() + tol))
+    within(dbias, want_bias, (M + 2) * F32 * dz.abs().sum(0))
+    plain_a, _, plain_bias = pf.gemm_bias_gelu_backward(dc, b, pf.Checkpoint(None, None, saved.grad_codes), need=("dA", "dbias"))
+    tol = (BF + (N + 2) * 2.0 ** -23) * (dz.abs() @ b.double().abs().t())
+    within(plain_a, want_a, tol + BF * (want_a.abs() + tol))
+    assert torch.equal(plain_bias, dbias)
+
+
+@pytest.mark.parametrize("M,N,K", [(8, 64, 40), (9, 520, 264)])
+def test_backward_of_gradients_near_the_largest(M, N, K):
+    """dz = dC d is finite up to bf16's 3.39e38, whatever dC times a code on the way to it would be."""
+    saved = saved_of(M, N, K)
+    codes = torch.randint(0, 227, (M, N), dtype=torch.uint8, device=DEV, generator=torch.Generator(device=DEV).manual_seed(8))
+    codes[:, 1], codes[:, 2], codes[1:, 3] = 226, 0, 252  # d = 1, -0.13 and 1.13
+    saved = saved._replace(a_scale=torch.full((M,), 2.0 ** -30, device=DEV), grad_codes=codes)
+    dc = randn(M, N, seed=1).clamp(-3, 3) * 3e35
+    dc[0] = 3.3e38  # with the others' 8 * 1.02e36 below fp32's 3.40e38: dbias is finite
+    dc[0, ::2] *= -1
+    b = (randn(K, N, seed=2) * 2.0 ** -30).bfloat16()
+    check_backward(dc.bfloat16(), b, saved)
