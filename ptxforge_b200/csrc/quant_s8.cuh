@@ -59,15 +59,18 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
 
 // The input's scale split into s = m 2^e, so that the backward pass rounds once where it could round twice: the
 // tensor cores take q 2^e, which is exact in bf16 (7 bits), and round(m dz), whose product is q s dz; dA, which
-// has no use for m, is divided by it at the end.  1 <= m < 2, so a token of tiny or no input keeps its dA.  A scale
-// that is not finite goes to e alone: dB is NaN then, dA is not.
+// has no use for m, is divided by it at the end.  1/2 <= m < 1, so a token of tiny or no input keeps its dA, and m dz is
+// finite where dz is; but 1 <= m < 2 from 2^121 on (inputs past 3.376e38), where 127 2^e would not be finite otherwise.  A
+// scale that is not finite goes to e alone: dB is NaN then, dA is not.
 struct SplitScale {
   float m, e;
 };
 __device__ __forceinline__ SplitScale split_scale(float s) {
   const uint32_t b = __float_as_uint(s), field = b & 0x7F800000u;
   if (field == 0u || field == 0x7F800000u) return {1.f, field == 0u ? s : __uint_as_float(0x7FC00000u)};
-  return {__uint_as_float((b & 0x007FFFFFu) | 0x3F800000u), __uint_as_float(b & 0xFF800000u)};
+  const bool below = field < (121u + 127u) << 23;
+  return {__uint_as_float((b & 0x007FFFFFu) | (below ? 0x3F000000u : 0x3F800000u)),
+          __uint_as_float((b & 0xFF800000u) + (below ? 1u << 23 : 0u))};
 }
 
 // The whole numbers that four codes in a word stand for: grad codes code - 26 (NaN for 255) in steps of 1 or of 1 / 256,

@@ -138,3 +138,38 @@ def test_backward_of_gradients_near_the_largest(M, N, K):
     dc[0, ::2] *= -1
     b = (randn(K, N, seed=2) * 2.0 ** -30).bfloat16()
     check_backward(dc.bfloat16(), b, saved)
+
+
+@pytest.mark.parametrize("M,N,K", [(8, 64, 40), (9, 520, 264), (300, 2056, 264)])
+@pytest.mark.parametrize("scale", [1.99 * 2.0 ** -30, 1.0, 1.5, 1.99 * 2.0 ** -126, 2.0 ** -126])
+def test_backward_of_gradients_near_the_largest_with_any_scale(M, N, K, scale):
+    """The input's scale takes no part in dA, and dz near bf16's largest is finite with any of its mantissas."""
+    saved = saved_of(M, N, K)
+    saved = saved._replace(a_scale=torch.full((M,), scale, device=DEV), grad_codes=torch.full((M, N), 226, dtype=torch.uint8, device=DEV))
+    if scale >= 1:  # dB = q s dz stays finite
+        saved = saved._replace(a_codes=(saved.a_codes == 127).to(torch.int8))
+        saved.a_codes[1:] = 0
+    dc = torch.zeros(M, N, device=DEV)
+    dc[0] = 3.3e38 / max(scale, 1.0)
+    dc[0, ::3] = 1.8e38 / max(scale, 1.0)
+    dc[M // 2, 1::4] = -3e38 / max(scale, 1.0)
+    b = (randn(K, N, seed=2) * 2.0 ** -30).bfloat16()
+    check_backward(dc.bfloat16(), b, saved)
+
+
+@pytest.mark.parametrize("scale", [1.01 * 2.0 ** -7, 1.0, 1.99])
+def test_backward_of_gradients_near_the_smallest(scale):
+    """dz and dz times a scale's mantissa keep an absolute half step of bf16's smallest, 2^-134, below its normal range."""
+    M, N, K = 40, 136, 72
+    saved = saved_of(M, N, K)
+    saved = saved._replace(a_scale=torch.full((M,), scale, device=DEV))
+    dc = (randn(M, N, seed=1) * 2.0 ** -125).bfloat16()
+    b = (randn(K, N, seed=2) * 2.0 ** 30).bfloat16()
+    dz, a, want_a, want_b, want_bias = grads64(dc, b, saved)
+    dA, dB, dbias = pf.gemm_bias_gelu_backward(dc, b, saved)
+    off = BF * dz.abs() + 2.0 ** -133  # a step of 2^-134 of m dz is up to two of dz
+    tol = off @ b.double().abs().t() + (N + 2) * 2.0 ** -23 * (dz.abs() @ b.double().abs().t())
+    within(dA, want_a, tol + BF * (want_a.abs() + tol))
+    tol = a.abs().t() @ off + (M + 3) * 2.0 ** -23 * (a.abs().t() @ dz.abs())
+    within(dB, want_b, tol + BF * (want_b.abs() + tol) + 2.0 ** -134)
+    within(dbias, want_bias, (M + 2) * F32 * dz.abs().sum(0) + M * 2.0 ** -149)
