@@ -279,7 +279,8 @@ int pf_dequantize_s8(int device, int rows, int cols, const signed char *codes, l
                      int axis, pf_dtype dst, void *X, long long ldx, void *stream, char *err, size_t err_len);
 
 /* C[r,c] = f( scale_a[r] * scale_b[c] * sum_k A[r,k] * B[k,c] + bias[c] ), A [M x K] and B [K x N] int8 codes, the
- * sum exact in 32-bit integers (hence K 1 to 131071), the rest in fp32, rounded once to `out` (PF_BF16 or PF_F32).
+ * sum exact in 32-bit integers (hence K 1 to 131071), the rest in fp32, rounded once to `out` (PF_BF16 or PF_F32).  The
+ * scales may be any: their product alone may be past fp32's range where its product with the sum is not.
  * bias may be NULL (none); f is gelu_tanh where `gelu` is nonzero, the identity otherwise.
  * Rows of A or B that do not start on 16-byte boundaries (the matrix, or its row stride) are copied to `workspace`
  * first: pf_gemm_s8_workspace(...) bytes, 256-byte aligned; 0 bytes (NULL) where both fit as they are. */

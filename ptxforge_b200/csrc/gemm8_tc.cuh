@@ -104,6 +104,17 @@ __device__ __forceinline__ float4 load_channels(const float *p, int n) {
   return make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
 }
 
+// A channel's scale as two factors, one of them 1: sum * first * (the token's scale) * last.  A scale below 1 goes first,
+// any other last, so that no product on the way leaves fp32's range where the value itself does not (the two scales'
+// own product may, and so may the sum times a large one).  Every kernel and every place in a tile takes this one order, so a
+// token's values do not depend on what else is in the call.  It costs 0.4 % of 16384 x 14336 x 4096 (610 -> 612 us in bursts)
+// and, where the epilogue is all, 3 % with GELU and 6 % without (8192^2 x 256: 70.1 -> 72.3, 53.2 -> 56.5) beside scales
+// multiplied before the sum is there.
+struct ChannelScale {
+  float first, last;
+  __device__ __forceinline__ explicit ChannelScale(float s) : first(fabsf(s) < 1.f ? s : 1.f), last(fabsf(s) < 1.f ? 1.f : s) {}
+};
+
 template <class Out>
 struct EpilogueS8 {
   struct Args {
@@ -117,10 +128,10 @@ struct EpilogueS8 {
   const Args &a;
   const int c;
   const bool inside;
-  float sb, bias;
+  const ChannelScale sb;
+  float bias;
   __device__ __forceinline__ EpilogueS8(const Args &args, int channel, int channels)
-      : a(args), c(channel), inside(channel < channels) {
-    sb = inside ? a.sb[c] : 0.f;
+      : a(args), c(channel), inside(channel < channels), sb(channel < channels ? args.sb[channel] : 0.f) {
     bias = inside && a.bias ? a.bias[c] : 0.f;
   }
   static __device__ __forceinline__ float token(const Args &a, int t) { return a.sa[t]; }
@@ -128,8 +139,8 @@ struct EpilogueS8 {
   // Two tokens' sums and scalars -> their values.
   template <bool kGelu>
   __device__ __forceinline__ float2 value(uint32_t s0, uint32_t s1, float a0, float a1) const {
-    const float2 x = __ffma2_rn(make_float2(static_cast<float>(static_cast<int>(s0)), static_cast<float>(static_cast<int>(s1))),
-                                __fmul2_rn(make_float2(a0, a1), both(sb)), both(bias));
+    const float2 sum = make_float2(static_cast<float>(static_cast<int>(s0)), static_cast<float>(static_cast<int>(s1)));
+    const float2 x = __ffma2_rn(__fmul2_rn(__fmul2_rn(sum, both(sb.first)), make_float2(a0, a1)), both(sb.last), both(bias));
     return kGelu ? gelu_of(x) : x;
   }
   __device__ __forceinline__ void put(uint32_t sum, int t, float sa) const {
@@ -165,8 +176,10 @@ struct EpilogueS8 {
     }
     __device__ __forceinline__ void put(const uint32_t (&v)[4], int t, float sa) const {
       const auto two = [&](uint32_t v0, uint32_t v1, float s0, float s1, float b0, float b1) {
-        const float2 x = __ffma2_rn(make_float2(static_cast<float>(static_cast<int>(v0)), static_cast<float>(static_cast<int>(v1))),
-                                    __fmul2_rn(both(sa), make_float2(s0, s1)), make_float2(b0, b1));
+        const ChannelScale c0(s0), c1(s1);
+        const float2 sum = make_float2(static_cast<float>(static_cast<int>(v0)), static_cast<float>(static_cast<int>(v1)));
+        const float2 x = __ffma2_rn(__fmul2_rn(__fmul2_rn(sum, make_float2(c0.first, c1.first)), both(sa)),
+                                    make_float2(c0.last, c1.last), make_float2(b0, b1));
         return a.gelu ? gelu_of(x) : x;
       };
       const float2 y0 = two(v[0], v[1], sb.x, sb.y, bias.x, bias.y), y1 = two(v[2], v[3], sb.z, sb.w, bias.z, bias.w);

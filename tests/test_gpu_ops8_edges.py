@@ -173,3 +173,37 @@ def test_backward_of_gradients_near_the_smallest(scale):
     tol = a.abs().t() @ off + (M + 3) * 2.0 ** -23 * (a.abs().t() @ dz.abs())
     within(dB, want_b, tol + BF * (want_b.abs() + tol) + 2.0 ** -134)
     within(dbias, want_bias, (M + 2) * F32 * dz.abs().sum(0) + M * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("M,N,K", [(25, 25, 64), (25, 1025, 2048), (2500, 2050, 64)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_products_of_far_scales(M, N, K, dtype):
+    """Scales whose product alone is past fp32's range, times a sum that brings the value back into it (or is 0)."""
+    a, b, _, _, _ = s8_operands(M, N, K, seed=N)
+    a[:M // 2] = a[:M // 2].clamp(-1, 1)
+    a[3] = 0
+    each = torch.tensor([2.0 ** -126, 1e-30, 3e-20, 1e-9, 0.7, 1.0, 3e7, 1e18, 1e31, 2.6e36], device=DEV)
+    sa, sb = each[torch.arange(M, device=DEV) % 10], each[torch.arange(N, device=DEV) // 10 % 10]
+    want = a.double() @ b.double() * sa.double()[:, None] * sb.double()
+    c = pf.gemm_s8(a, b, sa, sb, dtype=dtype)
+    u = BF if dtype == torch.bfloat16 else 2.0 ** -24
+    fits = (want.abs() >= 2.0 ** -126) & (want.abs() < 3.3e38) | (want == 0)
+    assert fits.float().mean() > 0.4
+    tol = 4 * 2.0 ** -24 * want.abs()
+    within(c[fits], want[fits], (tol + u * (want.abs() + tol))[fits])
+    # below the smallest normal number an absolute half step and a rounding before it; above the largest, infinity
+    small, large = want.abs() < 2.0 ** -126, want.abs() > 3.45e38
+    assert ((c.double() - want).abs()[small] <= 2.0 ** -133).all() and torch.isinf(c[large]).all()
+
+
+@pytest.mark.parametrize("N,K", [(1001, 2048), (2056, 512), (4104, 4096)])
+def test_a_token_gets_the_same_bits_in_every_batch(N, K):
+    """The integer sums are exact and the rest goes by value: neither the number of tokens, and so the kernel, nor a token's
+    place among them moves a bit."""
+    a, b, sa, sb, bias = s8_operands(2500, N, K, seed=N)
+    sa[::7] *= 1e30
+    for gelu in (False, True):
+        c = pf.gemm_s8(a, b, sa, sb, bias, gelu=gelu, dtype=torch.float32)
+        for first, last in ((0, 1), (3, 4), (1, 18), (5, 45), (2, 131), (700, 1003), (11, 1211), (1, 2500)):
+            part = pf.gemm_s8(a[first:last], b, sa[first:last], sb, bias, gelu=gelu, dtype=torch.float32)
+            assert torch.equal(part, c[first:last])
