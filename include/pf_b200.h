@@ -316,9 +316,13 @@ size_t pf_gemm_bias_gelu_backward_workspace(int M, int N, int K);
 int pf_dequantize_gelu_grad(int device, long long count, const unsigned char *codes, pf_dtype dst, void *X,
                             void *stream, char *err, size_t err_len);
 
-/* Synchronise the device, read and clear the bits of bounded waits that ran out in this section's kernels (0 =
- * clean; bits as pf_device_status).  Bits of calls on every stream of the device gather in one word. */
+/* Synchronise the device, read the bits of bounded waits that ran out in this section's kernels (0 = clean; bits as
+ * pf_device_status), and clear those that were read.  Bits of calls on every stream of the device gather in one word. */
 int pf_ops8_status(int device, unsigned *err_word, char *err, size_t err_len);
+
+/* Self-test of these waits: launches one block that waits on an mbarrier nothing arrives at, bounded by `timeout_ns` (at
+ * most 10^10), and returns at once; pf_ops8_status reads the bit that it sets. */
+int pf_ops8_selftest_wait_timeout(int device, unsigned long long timeout_ns, void *stream, char *err, size_t err_len);
 
 /* ---- utilities ---------------------------------------------------------------------------- */
 

@@ -37,7 +37,7 @@ SYMBOLS = ("pf_open", "pf_close", "pf_prepare", "pf_bind", "pf_launch", "pf_time
            "pf_set_stream_k", "pf_run_host_rows", "pf_set_host_chunks",
            "pf_quantize_s8", "pf_dequantize_s8", "pf_gemm_s8", "pf_gemm_s8_workspace",
            "pf_gemm_bias_gelu_checkpoint", "pf_gemm_bias_gelu_backward", "pf_gemm_bias_gelu_backward_workspace", "pf_dequantize_gelu_grad",
-           "pf_ops8_status")
+           "pf_ops8_status", "pf_ops8_selftest_wait_timeout")
 
 
 class Tile(ctypes.Structure):
@@ -187,12 +187,14 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.pf_gemm_bias_gelu_backward_workspace.restype = sz
         lib.pf_dequantize_gelu_grad.argtypes = [i, ll, vp, i, vp, vp, text, sz]
         lib.pf_ops8_status.argtypes = [i, ctypes.POINTER(ctypes.c_uint), text, sz]
+        lib.pf_ops8_selftest_wait_timeout.argtypes = [i, ctypes.c_ulonglong, vp, text, sz]
         for name in ("pf_open", "pf_close", "pf_prepare", "pf_bind", "pf_launch", "pf_time", "pf_attrs",
                      "pf_device_status", "pf_set_wait_timeout", "pf_run_host", "pf_run_host_rows", "pf_shard_rows",
                      "pf_selftest_wait_timeout", "pf_upload", "pf_download", "pf_gemm_bias_gelu_noalloc",
                      "pf_prepare_image", "pf_time_cublas", "pf_set_stream_k", "pf_set_host_chunks",
                      "pf_quantize_s8", "pf_dequantize_s8", "pf_gemm_s8", "pf_gemm_bias_gelu_checkpoint",
-                     "pf_gemm_bias_gelu_backward", "pf_dequantize_gelu_grad", "pf_ops8_status"):
+                     "pf_gemm_bias_gelu_backward", "pf_dequantize_gelu_grad", "pf_ops8_status",
+                     "pf_ops8_selftest_wait_timeout"):
             getattr(lib, name).restype = ctypes.c_int
         if path is None:
             _lib = lib

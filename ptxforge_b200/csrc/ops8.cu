@@ -17,12 +17,15 @@
 #include "gemm8_tc.cuh"
 #include "host_util.cuh"
 #include "ops8_epilogue.cuh"
+#include "selftest.cuh"
 
-// Bounded waits that ran out, of every kernel here: bits are only ever set, until pf_ops8_status clears them, so calls
-// that overlap on the GPU may share it.
+// Bounded waits that ran out, of every kernel here: bits are only ever set, until pf_ops8_status clears those that it has
+// read, so calls that overlap on the GPU, and with that, may share it.
 static __device__ unsigned ops8_status_word;
 
 namespace {
+
+__global__ void clear_bits(unsigned *word, unsigned bits) { atomicAnd(word, ~bits); }
 
 using pf::DeviceGuard;
 typedef __nv_bfloat16 bf16;
@@ -745,8 +748,26 @@ int pf_ops8_status(int device, unsigned *err_word, char *err_text, size_t err_le
   DeviceGuard g(device);
   cudaError_t e = cudaDeviceSynchronize();
   if (e == cudaSuccess) e = cudaMemcpy(err_word, d->status, sizeof *err_word, cudaMemcpyDeviceToHost);
-  if (e == cudaSuccess) e = cudaMemset(d->status, 0, sizeof *err_word);
+  if (e == cudaSuccess && *err_word) {  // those alone: a kernel may have set another since
+    clear_bits<<<1, 1>>>(d->status, *err_word);
+    e = cudaGetLastError();
+  }
   return e == cudaSuccess ? PF_OK : err(PF_ECUDA, "status read: %s", cudaGetErrorString(e));
+}
+
+int pf_ops8_selftest_wait_timeout(int device, unsigned long long timeout_ns, void *stream, char *err_text, size_t err_len) {
+  const Err err{err_text, err_len};
+  if (err_text && err_len) err_text[0] = '\0';
+  if (timeout_ns == 0 || timeout_ns > pf::kSelftestMostNs)
+    return err(PF_EINVAL, "timeout_ns must be 1 to %llu (got %llu)", pf::kSelftestMostNs, timeout_ns);
+  Device *d;
+  cudaStream_t s;
+  int rc;
+  if ((rc = device_of(device, err, &d))) return rc;
+  DeviceGuard g(device);
+  if ((rc = stream_of(device, stream, err, &s))) return rc;
+  pf::selftest_wait_kernel<<<1, 32, 0, s>>>(d->status, timeout_ns);
+  return launched(err);
 }
 
 }  // extern "C"

@@ -28,6 +28,7 @@
 #include "gemm_tc2.cuh"
 #include "gemm_tc2w.cuh"
 #include "gemm_tf32x3.cuh"
+#include "selftest.cuh"
 
 #ifndef PF_VERSION_STR
 #define PF_VERSION_STR "0.1.0"
@@ -1319,29 +1320,12 @@ int pf_shard_rows(int M, int G, int g, int align, int *row0, int *rows) {
 // ------------------------------------------------------------------------------------------------
 // Bounded-wait self-test: one block waits on an mbarrier that nothing arrives at.
 // ------------------------------------------------------------------------------------------------
-namespace {
-__global__ void selftest_wait_kernel(unsigned *status, unsigned long long timeout_ns) {
-  __shared__ uint64_t bar;
-  __shared__ int abort_flag;
-  if (threadIdx.x == 0) {
-    pf::mbar_init(&bar, 1);
-    abort_flag = 0;
-    pf::fence_mbar_init();
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    if (!pf::mbar_wait(&bar, 0, timeout_ns, &abort_flag)) atomicOr(status, pf::kErrEpilogueWait);
-  }
-  __syncthreads();
-}
-}  // namespace
-
 extern "C" int pf_selftest_wait_timeout(pf_ctx *c, unsigned long long timeout_ns, unsigned *err_word) {
-  if (!c || !err_word || timeout_ns == 0 || timeout_ns > 10000000000ull)
+  if (!c || !err_word || timeout_ns == 0 || timeout_ns > pf::kSelftestMostNs)
     return set_err(c, PF_EINVAL, "bad self-test arguments");
   DeviceGuard g(c->device);
   PF_CUDA(c, cudaMemsetAsync(c->d_status, 0, sizeof(unsigned), c->stream));
-  selftest_wait_kernel<<<1, 32, 0, c->stream>>>(c->d_status, timeout_ns);
+  pf::selftest_wait_kernel<<<1, 32, 0, c->stream>>>(c->d_status, timeout_ns);
   PF_CUDA(c, cudaGetLastError());
   return pf_device_status(c, err_word);
 }

@@ -1,5 +1,9 @@
 """The 8-bit operators at the edges of their ranges and of their kernels' tiles, against their formulas in 64 bits (needs
 a B200: -m gpu).  Tolerances count roundings as test_gpu_ops8.py does."""
+import ctypes
+import threading
+import time
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -207,3 +211,45 @@ def test_a_token_gets_the_same_bits_in_every_batch(N, K):
         for first, last in ((0, 1), (3, 4), (1, 18), (5, 45), (2, 131), (700, 1003), (11, 1211), (1, 2500)):
             part = pf.gemm_s8(a[first:last], b, sa[first:last], sb, bias, gelu=gelu, dtype=torch.float32)
             assert torch.equal(part, c[first:last])
+
+
+# ---------------------------------------------------------------------------------------------
+# waits that ran out
+# ---------------------------------------------------------------------------------------------
+def run_out(stream, ns=1000):
+    """One bounded wait on `stream` that nothing ends."""
+    text = ctypes.create_string_buffer(256)
+    rc = pf.load_library().pf_ops8_selftest_wait_timeout(0, ns, stream.cuda_stream, text, 256)
+    assert rc == pf.PF_OK, text.value
+
+
+def test_a_wait_that_ran_out_is_reported_once():
+    run_out(torch.cuda.current_stream())
+    assert pf.ops8_status() != 0 and pf.ops8_status() == 0
+    q, s = pf.quantize_s8(randn(4, 64))  # the context stays usable
+    assert s.numel() == 4 and pf.ops8_status() == 0
+
+
+def test_no_report_is_lost_beside_a_thread_that_reads_them():
+    """A bit set while another thread reads and clears the word is seen by this read or by the next one."""
+    seen, stop, s = [], threading.Event(), torch.cuda.Stream()
+
+    def read():
+        while not stop.is_set():
+            if pf.ops8_status():
+                seen.append(1)
+
+    reader = threading.Thread(target=read)
+    reader.start()
+    try:
+        for i in range(500):
+            before = len(seen)
+            run_out(s)
+            s.synchronize()
+            limit = time.monotonic() + 1
+            while len(seen) == before and time.monotonic() < limit:
+                time.sleep(1e-5)
+            assert len(seen) > before, f"report {i} was lost"
+    finally:
+        stop.set()
+        reader.join()
