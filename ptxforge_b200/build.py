@@ -110,15 +110,22 @@ TORCH_LIB = os.path.join(HERE, "_ops8.so")
 
 
 def build_torch(force: bool = False) -> str | None:
-    """Build _ops8.so, the 8-bit operators' torch side (a Python module over libpf_b200.so), where torch is installed."""
+    """Build _ops8.so, the 8-bit operators' torch side (a Python module over libpf_b200.so), where there are a torch with
+    CUDA and a C++ compiler; the library itself needs neither."""
     try:
+        import torch
         from torch.utils import cpp_extension
     except ImportError:
+        return None
+    cxx = shutil.which("g++")
+    if torch.version.cuda is None or cxx is None:
+        why = "this torch has no CUDA" if torch.version.cuda is None else "g++ not found"
+        print(f"_ops8.so (the 8-bit operators on torch tensors) is not built: {why}", file=sys.stderr)
         return None
     if force or _stale(TORCH_LIB, sorted(_includes(TORCH_SRC)) + [os.path.abspath(__file__)]):
         cuda = os.path.dirname(os.path.dirname(nvcc_path()))
         include = [INCLUDE, *cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
-        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", *(a for d in include for a in ("-isystem", d)), TORCH_SRC,
+        _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", *(a for d in include for a in ("-isystem", d)), TORCH_SRC,
               "-o", TORCH_LIB + ".tmp", *(a for d in cpp_extension.library_paths() for a in ("-L", d)), "-lc10", "-lc10_cuda",
               "-ltorch_cpu", "-ltorch", "-ltorch_python", "-L", HERE, "-lpf_b200", "-Wl,-rpath,$ORIGIN"])
         os.replace(TORCH_LIB + ".tmp", TORCH_LIB)

@@ -29,3 +29,35 @@ def test_selftest_of_the_waits_refuses_what_is_not_bounded():
     for ns in (0, 10 ** 10 + 1):
         text = ctypes.create_string_buffer(256)
         assert pf.load_library().pf_ops8_selftest_wait_timeout(0, ns, None, text, 256) == pf.PF_EINVAL and b"timeout_ns" in text.value
+
+
+# ---------------------------------------------------------------------------------------------
+# the build of the torch side
+# ---------------------------------------------------------------------------------------------
+@pytest.fixture
+def torch_build(monkeypatch, tmp_path):
+    """build_torch with its outputs in a folder of their own; the commands that it would run, which do nothing."""
+    commands = []
+
+    def run(cmd):
+        commands.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return ""
+
+    monkeypatch.setattr(pbuild, "_run", run)
+    monkeypatch.setattr(pbuild, "TORCH_LIB", str(tmp_path / "_ops8.so"))
+    monkeypatch.setattr(pbuild, "OBJ_DIR", str(tmp_path))
+    return commands
+
+
+def test_the_library_builds_beside_a_torch_without_cuda(torch_build, monkeypatch, capsys):
+    monkeypatch.setattr(torch.version, "cuda", None)
+    assert pbuild.build_torch() is None and not torch_build
+    assert "CUDA" in capsys.readouterr().err
+
+
+def test_the_library_builds_without_a_host_compiler_for_torch(torch_build, monkeypatch, capsys):
+    which = pbuild.shutil.which
+    monkeypatch.setattr(pbuild.shutil, "which", lambda name, *a, **k: None if name == "g++" else which(name, *a, **k))
+    assert pbuild.build_torch() is None and not torch_build
+    assert "g++" in capsys.readouterr().err
