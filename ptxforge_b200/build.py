@@ -122,13 +122,22 @@ def build_torch(force: bool = False) -> str | None:
         why = "this torch has no CUDA" if torch.version.cuda is None else "g++ not found"
         print(f"_ops8.so (the 8-bit operators on torch tensors) is not built: {why}", file=sys.stderr)
         return None
-    if force or _stale(TORCH_LIB, sorted(_includes(TORCH_SRC)) + [os.path.abspath(__file__)]):
+    # It fits one torch and one Python: another of either builds it again.
+    built_for, stamp = f"{torch.__version__} {sysconfig.get_config_var('SOABI')}", os.path.join(OBJ_DIR, "ops8_torch.txt")
+    same = False
+    if os.path.exists(stamp):
+        with open(stamp) as f:
+            same = f.read() == built_for
+    if force or not same or _stale(TORCH_LIB, sorted(_includes(TORCH_SRC)) + [os.path.abspath(__file__)]):
         cuda = os.path.dirname(os.path.dirname(nvcc_path()))
         include = [INCLUDE, *cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
         _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", *(a for d in include for a in ("-isystem", d)), TORCH_SRC,
               "-o", TORCH_LIB + ".tmp", *(a for d in cpp_extension.library_paths() for a in ("-L", d)), "-lc10", "-lc10_cuda",
               "-ltorch_cpu", "-ltorch", "-ltorch_python", "-L", HERE, "-lpf_b200", "-Wl,-rpath,$ORIGIN"])
         os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+        os.makedirs(OBJ_DIR, exist_ok=True)
+        with open(stamp, "w") as f:
+            f.write(built_for)
     return TORCH_LIB
 
 

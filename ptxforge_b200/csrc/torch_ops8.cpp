@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/utils/pybind.h>
+#include <torch/version.h>
 
 #include <climits>
 #include <optional>
@@ -273,6 +274,7 @@ unsigned ops8_status(int device) {
 }  // namespace
 
 PYBIND11_MODULE(_ops8, m) {
+  m.attr("torch_version") = TORCH_VERSION;
   m.def("quantize_s8", &quantize_s8);
   m.def("dequantize_s8", &dequantize_s8);
   m.def("gemm_s8", &gemm_s8);

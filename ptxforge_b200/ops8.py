@@ -19,6 +19,7 @@ device wait ran out.  The checks and calls themselves are compiled (csrc/torch_o
 """
 from __future__ import annotations
 
+import re
 from typing import NamedTuple
 
 import ptxforge_b200 as _pf
@@ -30,11 +31,14 @@ def _ops():
     """The compiled side, loaded by the first call (the package itself loads without torch)."""
     global _module
     if _module is None:
-        import torch  # noqa: F401  (its libraries come first)
+        import torch  # its libraries come first
         try:
             from . import _ops8
         except ImportError as e:
             raise RuntimeError(f"ptxforge_b200/_ops8.so cannot be loaded ({e}): build it with `python -m ptxforge_b200.build`") from e
+        if re.match(r"\d+\.\d+\.\d+", torch.__version__)[0] != _ops8.torch_version:
+            raise RuntimeError(f"ptxforge_b200/_ops8.so was built for torch {_ops8.torch_version}, this is {torch.__version__}: "
+                               "build it again with `python -m ptxforge_b200.build`")
         _module = _ops8
     return _module
 

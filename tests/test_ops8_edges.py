@@ -61,3 +61,27 @@ def test_the_library_builds_without_a_host_compiler_for_torch(torch_build, monke
     monkeypatch.setattr(pbuild.shutil, "which", lambda name, *a, **k: None if name == "g++" else which(name, *a, **k))
     assert pbuild.build_torch() is None and not torch_build
     assert "g++" in capsys.readouterr().err
+
+
+def test_the_torch_side_is_built_again_for_another_torch_or_python(torch_build, monkeypatch):
+    assert pbuild.build_torch() and len(torch_build) == 1
+    assert pbuild.build_torch() and len(torch_build) == 1  # nothing changed
+    monkeypatch.setattr(torch, "__version__", "9.8.7+cu999")
+    assert pbuild.build_torch() and len(torch_build) == 2
+    assert pbuild.build_torch() and len(torch_build) == 2
+    var = pbuild.sysconfig.get_config_var
+    monkeypatch.setattr(pbuild.sysconfig, "get_config_var", lambda name: "cpython-399" if name == "SOABI" else var(name))
+    assert pbuild.build_torch() and len(torch_build) == 3
+
+
+def test_a_torch_side_of_another_torch_is_refused(monkeypatch):
+    from ptxforge_b200 import ops8
+    monkeypatch.setattr(ops8, "_module", None)
+    monkeypatch.setattr(torch, "__version__", "9.8.7+cu999")
+    with pytest.raises(RuntimeError, match="9.8.7.*ptxforge_b200.build"):
+        ops8.quantize_s8(torch.zeros(2, 4))
+    monkeypatch.undo()
+    monkeypatch.setattr(ops8, "_module", None)
+    monkeypatch.setattr(torch, "__version__", re.match(r"[\d.]+", torch.__version__)[0] + "a0+git123")
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        ops8.quantize_s8(torch.zeros(2, 4))
