@@ -76,11 +76,13 @@ class Checkpoint(NamedTuple):
     grad_codes: object  # uint8 [M, N]
 
     def input(self, dtype=None):
-        """The input as the backward pass sees it, in `dtype` (default bfloat16)."""
+        """The input as the backward pass sees it, in `dtype` (default bfloat16), on torch's current stream."""
+        if self.a_codes is None:
+            raise ValueError("the checkpoint was made with keep_input=False: it has no input")
         return dequantize_s8(self.a_codes, self.a_scale, dtype=dtype)
 
     def gelu_grad(self, dtype=None):
-        """The GELU's derivative as the backward pass sees it, in `dtype` (default bfloat16)."""
+        """The GELU's derivative as the backward pass sees it, in `dtype` (default bfloat16), on torch's current stream."""
         return dequantize_gelu_grad(self.grad_codes, dtype=dtype)
 
 

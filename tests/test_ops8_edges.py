@@ -85,3 +85,9 @@ def test_a_torch_side_of_another_torch_is_refused(monkeypatch):
     monkeypatch.setattr(torch, "__version__", re.match(r"[\d.]+", torch.__version__)[0] + "a0+git123")
     with pytest.raises(ValueError, match="CUDA tensor"):
         ops8.quantize_s8(torch.zeros(2, 4))
+
+
+def test_a_checkpoint_without_its_input_says_so():
+    import ptxforge_b200 as pf
+    with pytest.raises(ValueError, match="keep_input=False"):
+        pf.Checkpoint(None, None, torch.zeros(4, 8, dtype=torch.uint8)).input()
