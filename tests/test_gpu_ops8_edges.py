@@ -9,7 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import ptxforge_b200 as pf  # noqa: E402
-from test_gpu_ops8 import (BF, DEV, F32, check_s8, gelu64, grad64, grads64, layer, no_wait_ran_out,  # noqa: E402,F401
+from test_gpu_ops8 import (BF, DEV, F32, check_s8, codes64, gelu64, grad64, grads64, layer, no_wait_ran_out,  # noqa: E402,F401
                            randn, s8_operands, saved_of, within)
 
 pytestmark = pytest.mark.gpu
@@ -253,3 +253,95 @@ def test_no_report_is_lost_beside_a_thread_that_reads_them():
     finally:
         stop.set()
         reader.join()
+
+
+# ---------------------------------------------------------------------------------------------
+# matrices of more than 2^31 values, and more tokens than a grid's second dimension has tiles
+# ---------------------------------------------------------------------------------------------
+@pytest.fixture
+def large():
+    """Memory of large tensors goes back to the device afterwards."""
+    yield
+    torch.cuda.empty_cache()
+
+
+def some_rows(rows, cols):
+    """The first rows, those around value 2^31, and the last ones."""
+    at = 2 ** 31 // cols
+    return sorted({0, 1, rows - 2, rows - 1} | {r for r in (at - 1, at, at + 1) if 0 <= r < rows})
+
+
+@pytest.mark.parametrize("rows,cols", [(65537, 32776), (1048577, 2049)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("axis", [1, 0])
+def test_store_past_2_to_the_31_values(rows, cols, dtype, axis, large):
+    assert rows * cols > 2 ** 31
+    x = torch.empty(rows, cols, dtype=dtype, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    x[rows - 1] *= 2  # the last row has most columns' largest values
+    codes, scale = pf.quantize_s8(x, axis)
+    back = pf.dequantize_s8(codes, scale, axis, dtype=dtype)
+    if axis == 0:
+        want_scale = torch.zeros(cols, device=DEV)
+        for first in range(0, rows, 16384):
+            want_scale = torch.maximum(want_scale, x[first:first + 16384].float().abs().amax(0))
+        want_scale = (want_scale.double() / 127).float()
+        assert torch.equal(scale, want_scale)
+    for r in some_rows(rows, cols):
+        if axis == 1:
+            want, s = codes64(x[r:r + 1], 1)
+            assert torch.equal(scale[r:r + 1], s)
+        else:
+            s = scale
+            want = torch.round(x[r:r + 1].double() / s.double()).to(torch.int8)
+        assert torch.equal(codes[r:r + 1], want)
+        assert torch.equal(back[r], (want[0].float() * s).to(dtype))
+
+
+def test_derivatives_past_2_to_the_31(large):
+    n = 2 ** 31 + 4333
+    codes = torch.zeros(n, dtype=torch.uint8, device=DEV)
+    ends = torch.tensor([0, 1, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 1, n - 4097, n - 2, n - 1], device=DEV)
+    codes[ends] = torch.arange(100, 108, dtype=torch.uint8, device=DEV)
+    d = pf.dequantize_gelu_grad(codes)
+    want = ((torch.arange(100, 108, device=DEV).double() - 26) / 200).float().bfloat16()
+    assert torch.equal(d[ends], want)
+    assert int((d == torch.tensor(-0.13, device=DEV).bfloat16()).sum()) == n - 8
+
+
+@pytest.mark.parametrize("M,N,K", [(2 ** 21 + 77, 1032, 16), (2 ** 21 + 77, 1033, 17),  # C past 2^31 values
+                                   (65537, 16, 32784),                                  # A past it
+                                   (40, 65537 * 16, 2064),                              # B past it
+                                   (8388481, 16, 16)])                                  # 65,536 tiles of 128 tokens
+def test_product_past_2_to_the_31_values(M, N, K, large):
+    a, b, sa, sb, bias = s8_operands(M, N, K, seed=3)
+    c = pf.gemm_s8(a, b, sa, sb, bias)
+    rows = some_rows(M, min(N, 2 ** 30)) if M > 40 else [0, 17, 39]
+    rows = sorted(set(rows) | {M // 2, max(0, M - 300)})
+    check_s8(c[rows], a[rows], b, sa[rows], sb, bias, False)
+
+
+@pytest.mark.parametrize("M,N,K", [(2 ** 21 + 77, 1032, 16), (2 ** 21 + 77, 16, 1032), (8388481, 8, 8)])
+def test_a_layer_past_2_to_the_31_values(M, N, K, large):
+    a, b, bias = layer(M, N, K, seed=4)
+    c, saved = pf.gemm_bias_gelu_checkpoint(a, b, bias)
+    rows = sorted(set(some_rows(M, max(N, K))) | {M // 2, M - 300})
+    z = a[rows].double() @ b.double() + bias.double()
+    dz = (K + 3) * 2.0 ** -23 * (a[rows].double().abs() @ b.double().abs() + bias.double().abs())
+    y = gelu64(z)
+    within(c[rows], y, 1.13 * dz + 2.0 ** -20 * (1 + y.abs()) + BF * (y.abs() + 1.13 * dz))
+    part = pf.Checkpoint(*(t[rows] for t in saved))
+    within(part.gelu_grad(torch.float32), grad64(z), 0.0025 + 1.13 * dz + 2.0 ** -18)
+    want, want_scale = codes64(a[rows], 1)
+    assert torch.equal(part.a_codes, want) and torch.equal(part.a_scale, want_scale)
+    # a gradient in these rows alone, so that they are all there is to sum
+    dc = torch.zeros_like(c)
+    dc[rows] = randn(len(rows), N, seed=5, dtype=torch.bfloat16)
+    dA, dB, dbias = pf.gemm_bias_gelu_backward(dc, b, saved)
+    dz, x, want_a, want_b, want_bias = grads64(dc[rows], b, part)
+    tol = (BF + (N + 2) * 2.0 ** -23) * (dz.abs() @ b.double().abs().t())
+    within(dA[rows], want_a, tol + BF * (want_a.abs() + tol))
+    tol = (BF + (len(rows) + 3) * 2.0 ** -23) * (x.abs().t() @ dz.abs())  # adding zeros rounds nothing
+    within(dB, want_b, tol + BF * (want_b.abs() + tol))
+    within(dbias, want_bias, (len(rows) + 2) * F32 * dz.abs().sum(0))
+    dA[rows] = 0
+    assert not dA.any()
