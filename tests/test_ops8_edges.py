@@ -91,3 +91,19 @@ def test_a_checkpoint_without_its_input_says_so():
     import ptxforge_b200 as pf
     with pytest.raises(ValueError, match="keep_input=False"):
         pf.Checkpoint(None, None, torch.zeros(4, 8, dtype=torch.uint8)).input()
+
+
+# ---------------------------------------------------------------------------------------------
+# registers of the CTA-pair kernels, as ptxas reports them
+# ---------------------------------------------------------------------------------------------
+def test_pair_kernels_fit_one_cta_per_sm():
+    pbuild.build()
+    log = os.path.join(os.path.dirname(pbuild.LIB), "libpf_b200.ptxas.txt")
+    if not os.path.exists(log):
+        pytest.skip("no ptxas report beside the library")
+    seen = []
+    for name, regs in re.findall(r"Function properties for (\S*gemm8_pair\S*)\n.*?Used (\d+) registers", open(log).read(), re.S):
+        warps = 2 + int(re.search(r"gemm8_pairILi\d+ELi(\d+)E", name)[1])  # producer, MMA and the epilogue warps
+        seen.append(warps)
+        assert -(-int(regs) * 32 // 512) * 512 * warps <= 65536, (name, regs, warps)  # registers come in blocks of 512 a warp
+    assert set(seen) == {10, 18} and len(seen) >= 10
