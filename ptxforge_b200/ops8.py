@@ -11,11 +11,12 @@ Training: the bf16 fused product with its activations kept in 8 bits for the bac
     C, saved = pf.gemm_bias_gelu_checkpoint(A, B, bias)
     dA, dB, dbias = pf.gemm_bias_gelu_backward(dC, B, saved)
 
-Matrices have contiguous rows; a row stride above the row's length is fine where a function says so.  Operands that
-do not fit raise ValueError before anything is launched, what the library refuses raises PFError.  Work goes on
-`stream` (a torch stream or a handle), by default torch's current stream of the operands' device; outputs and workspaces
-that a call makes are allocated on that stream.  Calls do not wait for the GPU: ops8_status() says whether a bounded
-device wait ran out.  The checks and calls themselves are compiled (csrc/torch_ops8.cpp).
+Matrices have contiguous rows; a row stride above the row's length is fine where a function says so.  Results that a
+caller passes overlap no operand.  Operands that do not fit raise ValueError before anything is launched, what the
+library refuses raises PFError.  Work goes on `stream` (a torch stream or a handle), by default torch's current stream of
+the operands' device; outputs and workspaces that a call makes are allocated on that stream.  Calls do not wait for the
+GPU: ops8_status() says whether a bounded device wait ran out.  The checks and calls themselves are compiled
+(csrc/torch_ops8.cpp).
 """
 from __future__ import annotations
 
@@ -89,7 +90,7 @@ class Checkpoint(NamedTuple):
 def gemm_bias_gelu_checkpoint(A, B, bias, C=None, *, keep_input: bool = True, stream=None):
     """(C, checkpoint): C = gelu_tanh(A @ B + bias) in bfloat16, for bfloat16 A [M, K] and B [K, N] and float32 bias [N],
     and in 8 bits what gemm_bias_gelu_backward needs.  keep_input=False leaves the input out (no dB then).  Operands
-    contiguous, N and K multiples of 8."""
+    contiguous and 16-byte aligned, N and K multiples of 8."""
     C, a_codes, a_scale, grad_codes = _ops().gemm_bias_gelu_checkpoint(A, B, bias, C, keep_input, _handle(stream))
     return C, Checkpoint(a_codes, a_scale, grad_codes)
 
@@ -97,7 +98,7 @@ def gemm_bias_gelu_checkpoint(A, B, bias, C=None, *, keep_input: bool = True, st
 def gemm_bias_gelu_backward(dC, B, checkpoint: Checkpoint, *, need=("dA", "dB", "dbias"), stream=None):
     """(dA, dB, dbias) of C = gelu_tanh(A @ B + bias) from dC [M, N] (bfloat16), B and the forward pass's checkpoint:
     bfloat16 [M, K] and [K, N], float32 [N]; None for those that `need` leaves out.  Sums are in float32, in an order
-    that depends on the sizes alone."""
+    that depends on the sizes and on `need` alone.  Operands contiguous."""
     unknown = set(need) - {"dA", "dB", "dbias"}
     if unknown:
         raise ValueError(f"need names dA, dB and dbias, got {sorted(unknown)}")
