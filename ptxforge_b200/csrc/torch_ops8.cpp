@@ -91,6 +91,31 @@ float *vector(const Tensor &x, const char *name, int64_t n, int device) {
   return static_cast<float *>(x.data_ptr());
 }
 
+// Memory that a result which the caller passes must not share with an operand: some blocks of a kernel write while others
+// still read.  Rows of `width` bytes, `stride` apart.
+struct Rows {
+  uintptr_t first;
+  long long rows, width, stride;
+  Rows(const Tensor &x, const Matrix &m)
+      : first(reinterpret_cast<uintptr_t>(x.data_ptr())), rows(m.rows), width(m.cols * x.element_size()), stride(m.ld * x.element_size()) {}
+  explicit Rows(const Tensor &x)  // contiguous
+      : first(reinterpret_cast<uintptr_t>(x.data_ptr())), rows(1), width(x.numel() * x.element_size()), stride(width) {}
+  uintptr_t end() const { return first + (rows - 1) * stride + width; }
+};
+bool overlap(const Rows &a, const Rows &b) {
+  if (a.rows == 0 || a.width == 0 || b.rows == 0 || b.width == 0 || a.end() <= b.first || b.end() <= a.first) return false;
+  // Within one another's bounds they are apart only as columns beside one another: rows at the same distance, or a single
+  // row, that fit between the other's.
+  if (a.rows == 1 && b.rows == 1) return true;
+  if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
+  const long long stride = a.rows > 1 ? a.stride : b.stride;
+  const long long gap = (static_cast<long long>(b.first - a.first) % stride + stride) % stride;
+  return gap < a.width || gap + b.width > stride;
+}
+void apart(const Rows &result, const char *name, const Rows &operand, const char *other) {
+  if (overlap(result, operand)) refuse(name, " overlaps ", other);
+}
+
 // The stream of a call: the handle given, else torch's current one of the device.  Outputs and workspaces are allocated
 // on it, so that memory comes from work that is before the call and goes to work that is after it.
 class Place {
@@ -151,10 +176,16 @@ py::tuple quantize_s8(const Tensor &X, int axis, MaybeTensor codes, MaybeTensor 
   const Matrix x = matrix(X, "X", X.scalar_type(), -1);
   const int n = scales(axis, x), dev = X.get_device();
   const Place place(dev, handle);
+  const bool given = codes || scale;
   if (!codes) codes = place.empty({x.rows, x.cols}, ScalarType::Char);
   if (!scale) scale = place.empty({n}, ScalarType::Float);
   const Matrix q = matrix_of(*codes, "codes", ScalarType::Char, x.rows, x.cols, dev);
   float *s = vector(*scale, "scale", n, dev);
+  if (given) {
+    apart({*codes, q}, "codes", {X, x}, "X");
+    apart(Rows(*scale), "scale", {X, x}, "X");
+    apart(Rows(*scale), "scale", {*codes, q}, "codes");
+  }
   call("pf_quantize_s8", pf_quantize_s8, dev, src, x.rows, x.cols, static_cast<const void *>(X.data_ptr()), x.ld, axis, int8(*codes),
        q.ld, s, place.stream());
   return py::make_tuple(*codes, *scale);
@@ -167,8 +198,13 @@ Tensor dequantize_s8(const Tensor &codes, const Tensor &scale, int axis, MaybeTe
   const ScalarType type = type_of(dtype, out);
   const pf_dtype dst = type_code(type, "dtype");
   const Place place(dev, handle);
+  const bool given = out.has_value();
   if (!out) out = place.empty({q.rows, q.cols}, type);
   const Matrix x = matrix_of(*out, "out", type, q.rows, q.cols, dev);
+  if (given) {
+    apart({*out, x}, "out", {codes, q}, "codes");
+    apart({*out, x}, "out", Rows(scale), "scale");
+  }
   call("pf_dequantize_s8", pf_dequantize_s8, dev, q.rows, q.cols, static_cast<const signed char *>(int8(codes)), q.ld, s, axis, dst,
        out->data_ptr(), x.ld, place.stream());
   return *out;
@@ -186,8 +222,16 @@ Tensor gemm_s8(const Tensor &A, const Tensor &B, const Tensor &scale_a, const Te
   const ScalarType type = type_of(dtype, C);
   const pf_dtype out = type_code(type, "dtype");
   const Place place(dev, handle);
+  const bool given = C.has_value();
   if (!C) C = place.empty({M, N}, type);
   const Matrix c = matrix_of(*C, "C", type, M, N, dev);
+  if (given) {
+    apart({*C, c}, "C", {A, a}, "A");
+    apart({*C, c}, "C", {B, b}, "B");
+    apart({*C, c}, "C", Rows(scale_a), "scale_a");
+    apart({*C, c}, "C", Rows(scale_b), "scale_b");
+    if (bias) apart({*C, c}, "C", Rows(*bias), "bias");
+  }
   const signed char *pa = int8(A), *pb = int8(B);
   const size_t size = pf_gemm_s8_workspace(M, N, K, pa, a.ld, pb, b.ld);  // 0 where rows start on 16-byte boundaries
   Tensor space;  // back to the stream's pool on return
@@ -205,8 +249,14 @@ py::tuple gemm_bias_gelu_checkpoint(const Tensor &A, const Tensor &B, const Tens
   const int M = a.rows, N = b.cols, K = a.cols;
   const float *bi = vector(bias, "bias", N, dev);
   const Place place(dev, handle);
+  const bool given = C.has_value();
   if (!C) C = place.empty({M, N}, ScalarType::BFloat16);
   matrix_of(*C, "C", ScalarType::BFloat16, M, N, dev, true);
+  if (given) {
+    apart(Rows(*C), "C", Rows(A), "A");
+    apart(Rows(*C), "C", Rows(B), "B");
+    apart(Rows(*C), "C", Rows(bias), "bias");
+  }
   const Tensor d = place.empty({M, N}, ScalarType::Byte);
   MaybeTensor q, s;
   if (keep_input) {
@@ -260,6 +310,7 @@ Tensor dequantize_gelu_grad(const Tensor &codes, MaybeTensor out, const py::obje
   check(*out, "out", type, dev);
   if (out->sizes() != codes.sizes()) refuse("out must have codes' shape ", shape_name(codes), ", got ", shape_name(*out));
   if (!out->is_contiguous()) refuse("out must be contiguous");
+  apart(Rows(*out), "out", Rows(codes), "codes");
   call("pf_dequantize_gelu_grad", pf_dequantize_gelu_grad, dev, static_cast<long long>(codes.numel()),
        static_cast<const unsigned char *>(uint8(codes)), dst, out->data_ptr(), place.stream());
   return *out;

@@ -12,7 +12,7 @@ Training: the bf16 fused product with its activations kept in 8 bits for the bac
     dA, dB, dbias = pf.gemm_bias_gelu_backward(dC, B, saved)
 
 Matrices have contiguous rows; a row stride above the row's length is fine where a function says so.  Results that a
-caller passes overlap no operand.  Operands that do not fit raise ValueError before anything is launched, what the
+caller passes must not overlap an operand.  Operands that do not fit raise ValueError before anything is launched, what the
 library refuses raises PFError.  Work goes on `stream` (a torch stream or a handle), by default torch's current stream of
 the operands' device; outputs and workspaces that a call makes are allocated on that stream.  Calls do not wait for the
 GPU: ops8_status() says whether a bounded device wait ran out.  The checks and calls themselves are compiled

@@ -345,3 +345,70 @@ def test_a_layer_past_2_to_the_31_values(M, N, K, large):
     within(dbias, want_bias, (len(rows) + 2) * F32 * dz.abs().sum(0))
     dA[rows] = 0
     assert not dA.any()
+
+
+# ---------------------------------------------------------------------------------------------
+# results over operands
+# ---------------------------------------------------------------------------------------------
+def carve(raw, first, dtype, rows, cols, ld=None):
+    """A matrix (rows None: a vector) of `dtype` whose memory starts at byte `first` of `raw`, rows `ld` bytes apart."""
+    flat = raw[first:first + (raw.numel() - first) // 4 * 4].view(dtype)
+    if rows is None:
+        return flat[:cols]
+    return flat.as_strided((rows, cols), ((ld or cols * flat.element_size()) // flat.element_size(), 1))
+
+
+I8, U8, BF16, FP32 = torch.int8, torch.uint8, torch.bfloat16, torch.float32
+
+
+def product_into(v, C, scale_a=8192, scale_b=9216, bias=None):
+    """gemm_s8 of A at byte 0 and B at byte 4096 into C."""
+    return pf.gemm_s8(v(0, I8, 48, 64), v(4096, I8, 64, 64), v(scale_a, FP32, None, 48), v(scale_b, FP32, None, 64),
+                      bias and v(bias, FP32, None, 64), C)
+
+
+def layer_into(v, C, bias=16384):
+    return pf.gemm_bias_gelu_checkpoint(v(0, BF16, 48, 64), v(8192, BF16, 64, 64), v(bias, FP32, None, 64), v(C, BF16, 48, 64))
+
+
+@pytest.mark.parametrize("call", [
+    lambda v: pf.quantize_s8(v(0, BF16, 48, 64), codes=v(0, I8, 48, 64, 128), scale=v(8192, FP32, None, 48)),  # in place
+    lambda v: pf.quantize_s8(v(0, BF16, 48, 64), codes=v(64, I8, 48, 64, 128), scale=v(8192, FP32, None, 48)),
+    lambda v: pf.quantize_s8(v(0, BF16, 48, 64), codes=v(6080, I8, 48, 64), scale=v(16384, FP32, None, 48)),   # the last row
+    lambda v: pf.quantize_s8(v(0, FP32, 48, 64), codes=v(16384, I8, 48, 64), scale=v(12284, FP32, None, 48)),  # the last value
+    lambda v: pf.quantize_s8(v(0, FP32, 48, 64, 512), 0, codes=v(252, I8, 48, 64, 512), scale=v(32768, FP32, None, 64)),
+    lambda v: pf.quantize_s8(v(0, FP32, 48, 64), codes=v(16384, I8, 48, 64), scale=v(16384 + 3068, FP32, None, 48)),
+    lambda v: pf.dequantize_s8(v(0, I8, 48, 64, 128), v(8192, FP32, None, 48), out=v(0, BF16, 48, 64)),        # in place
+    lambda v: pf.dequantize_s8(v(0, I8, 48, 64), v(16384, FP32, None, 48), out=v(16384, BF16, 48, 64)),
+    lambda v: pf.dequantize_s8(v(0, I8, 1, 64), v(80, FP32, None, 1), out=v(64, BF16, 1, 64)),
+    lambda v: product_into(v, v(0, BF16, 48, 64)),
+    lambda v: product_into(v, v(4096, BF16, 48, 64, 256)),
+    lambda v: product_into(v, v(8380, FP32, 48, 64)),
+    lambda v: product_into(v, v(12288, BF16, 48, 64), scale_b=12288),
+    lambda v: product_into(v, v(16384, BF16, 48, 64), bias=16384 + 4096),
+    lambda v: layer_into(v, 0),
+    lambda v: layer_into(v, 8208),
+    lambda v: layer_into(v, 16384, bias=16640),
+    lambda v: pf.dequantize_gelu_grad(v(0, U8, None, 64), out=v(60, BF16, None, 64)),
+])
+def test_results_over_operands_are_refused(call):
+    raw = torch.zeros(1 << 16, dtype=torch.uint8, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        call(lambda *a: carve(raw, *a))
+
+
+def test_results_beside_operands_are_not():
+    """One buffer for all: columns beside one another, a single row between rows, the next byte."""
+    raw = torch.zeros(1 << 16, dtype=torch.uint8, device=DEV)
+    x = carve(raw, 0, BF16, 48, 64, 256)  # a row: 128 bytes of values, 64 of codes, 64 for others
+    x.copy_(randn(48, 64, dtype=BF16))
+    x0, (want, want_scale) = x.clone(), codes64(x, 1)
+    codes, scale = pf.quantize_s8(x, codes=carve(raw, 128, I8, 48, 64, 256), scale=carve(raw, 47 * 256 + 192, FP32, None, 48))
+    assert torch.equal(codes, want) and torch.equal(scale, want_scale) and torch.equal(x, x0)
+    one = pf.dequantize_s8(codes[:1, :32], scale[:1], out=carve(raw, 192, BF16, 1, 32))
+    assert torch.equal(one, (want[:1, :32].float() * want_scale[0]).to(BF16)) and torch.equal(x, x0) and torch.equal(codes, want)
+    a, b, bias = layer(48, 64, 64)
+    flat = torch.zeros(4 * 4096, dtype=BF16, device=DEV)
+    flat[:112 * 64] = torch.cat([a.flatten(), b.flatten()])
+    A, B, C = flat[:48 * 64].view(48, 64), flat[48 * 64:112 * 64].view(64, 64), flat[112 * 64:160 * 64].view(48, 64)
+    assert torch.equal(pf.gemm_bias_gelu_checkpoint(A, B, bias, C)[0], pf.gemm_bias_gelu_checkpoint(a, b, bias)[0])
