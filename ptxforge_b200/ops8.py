@@ -14,8 +14,9 @@ Training: the bf16 fused product with its activations kept in 8 bits for the bac
 Matrices have contiguous rows; a row stride above the row's length is fine where a function says so.  Results that a
 caller passes must not overlap an operand.  Operands that do not fit raise ValueError before anything is launched, what the
 library refuses raises PFError.  Work goes on `stream` (a torch stream or a handle), by default torch's current stream of
-the operands' device; outputs and workspaces that a call makes are allocated on that stream.  Calls do not wait for the
-GPU: ops8_status() says whether a bounded device wait ran out.  The checks and calls themselves are compiled
+the operands' device; outputs and workspaces that a call makes are allocated on that stream, and operands of another
+stream have to live until it has used them (Tensor.record_stream), as with torch's own functions.  Calls do not wait for
+the GPU: ops8_status() says whether a bounded device wait ran out.  The checks and calls themselves are compiled
 (csrc/torch_ops8.cpp).
 """
 from __future__ import annotations
