@@ -304,8 +304,8 @@ int pf_gemm_bias_gelu_checkpoint(int device, int M, int N, int K, const void *A,
 /* Its backward pass from dC [M x N] (bf16), B and the checkpoint:  dz = dC d,  dbias = sum over tokens of dz (fp32),
  * dA = dz B^T,  dB = A~^T dz with A~ = a_codes a_scale (bf16, fp32 sums).  Besides the results only dz
  * is rounded to bf16, once; dbias sums the unrounded dz.  dz is finite up to bf16's 3.39e38, half of that for tokens with
- * a_scale from 2^121 on (inputs past 3.376e38).  Any of dA, dB, dbias may be NULL (not wanted).  The same
- * inputs and wanted results give the same bits.  `workspace`: pf_gemm_bias_gelu_backward_workspace(M, N, K) bytes, 256-byte aligned. */
+ * a_scale from 2^121 on (inputs past 3.376e38).  Any of dA, dB, dbias may be NULL (not wanted).  The same inputs and wanted
+ * results give the same bits.  `workspace`: pf_gemm_bias_gelu_backward_workspace(M, N, K) bytes, 256-byte aligned. */
 int pf_gemm_bias_gelu_backward(int device, int M, int N, int K, const void *dC, const void *B,
                                const signed char *a_codes, const float *a_scale, const unsigned char *grad_codes,
                                void *dA, void *dB, float *dbias, void *workspace, size_t workspace_bytes, void *stream,
